@@ -401,6 +401,76 @@ int pd_gather(pd_comm* comm, pd_ctx* const* ctxs, int n_ctx, int root, void* rec
  * slice's used part are left as they were.  capacity: a multiple of 16; both addresses 16-byte aligned. */
 int pd_copy_used_skeletons(const void* src_dev, void* dst, int n_slices, uint64_t capacity, void* stream);
 
+/* ---- rows of scores: what a network answers that names one of many things per row ----
+ * No counterpart in the reference.  A row of scores (logits) over coordinate bins, classes or
+ * tokens is read out as pd_peaks reads a map: the scores of given answers, how sure the network
+ * is, the best answers with their scores; a row over experts as the experts that are to answer it,
+ * with their weights.  Equal scores go to the lower index everywhere.
+ *
+ * These calls need no context.  Pointers are device addresses on the current device; `stream` is
+ * a stream of it (NULL: the default stream).  A call enqueues kernels and nothing else (no memset,
+ * no copy, no allocation), so it can be captured; it does not wait.  Calls that overlap need
+ * workspaces of their own.  Logits are PD_F32, PD_BF16 or PD_F16, row r at logits + r * row_stride
+ * elements (row_stride 0: the same row each time), aligned to their type and no further.
+ * Everything else is float32 / int32 and contiguous; all sums and statistics are held in 32 bits
+ * or more.  Bad arguments: PD_E_INVALID, text by pd_last_error(NULL). */
+enum { PD_BF16 = 3, PD_F16 = 4 };
+#define PD_MAX_COLUMNS (1 << 24)
+#define PD_MAX_TOKENS 64
+#define PD_MAX_ALTERNATIVES 64
+#define PD_MAX_EXPERTS 1024
+#define PD_MAX_GROUPS 64
+#define PD_MAX_ROUTES 32
+
+/* Row r holds columns 0 .. n-1, n = widths[r] clamped to 0..columns (widths NULL: columns); what lies
+ * behind is not read and counts as -inf.  With m the row's largest score, S = sum exp(x_j - m):
+ *   logp[r][t]  = (x[tokens[r][t]] - m) - log S for tokens 0..n-1; -inf for a token the row does not
+ *                 hold; 0 for a negative one (not given).  int64, n_tokens a row, at most 64.
+ *   entropy[r]  = log S - sum exp(x_j - m) (x_j - m) / S.  May be NULL.
+ *   stats[r]    = { m, log S, entropy }, for the gradient.  May be NULL.
+ *   top_logp, top_index [r][top]: the top largest, in descending order, at most 64 and at most columns.
+ * A row with nothing above -inf: logp -inf, entropy 0, alternatives 0, 1, .. with -inf, stats
+ * { -inf, 0, 0 }.  A row that holds a NaN or +inf: NaN, alternatives -1.
+ * workspace: pd_token_logprobs_workspace bytes (0: none is needed), 16-byte aligned. */
+uint64_t pd_token_logprobs_workspace(int dtype, int64_t rows, int64_t columns, int top);
+int pd_token_logprobs(const void* logits, int dtype, int64_t rows, int64_t columns, int64_t row_stride,
+                      const int32_t* widths, const int64_t* tokens, int n_tokens, int top, float* logp,
+                      float* entropy, float* stats, float* top_logp, int32_t* top_index, void* workspace,
+                      uint64_t workspace_bytes, void* stream);
+
+/* The gradient with respect to the logits, of their type, every column of every row:
+ *   grad[r][j] = -p_j (sum_t grad_logp[r][t] + grad_entropy[r] (log p_j + entropy[r])) + sum over t with
+ *   tokens[r][t] = j of grad_logp[r][t],   p_j = exp(x_j - m - log S) from stats.
+ * Tokens that are not given contribute nothing; columns behind a row's width and empty rows get 0.
+ * grad_entropy may be NULL.  grad may be the logits themselves (same stride) or must not overlap them. */
+int pd_token_logprobs_grad(const void* logits, int dtype, int64_t rows, int64_t columns, int64_t row_stride,
+                           const int32_t* widths, const float* stats, const int64_t* tokens, int n_tokens,
+                           const float* grad_logp, const float* grad_entropy, void* grad, int64_t grad_stride,
+                           void* stream);
+
+/* Which `top` experts (at most 32 of at most 1024) answer row r, in descending order, and their weights.
+ * p = softmax of the row or 1 / (1 + exp(-x)).  The order is that of p + bias, without bias that of the
+ * logits, decided as in float64 (the kernels work in float32 and go over a row again in float64 where two
+ * scores are too close to tell).  With groups > 1 (at most 64, equal parts of consecutive experts) the
+ * top_groups best groups are chosen first, by their largest value (PD_GROUP_MAX) or the sum of their two
+ * largest of p, or p + bias (PD_GROUP_TOP2); only their experts are eligible.
+ *   weights[r][i] = scale * p_i, with renormalise scale * p_i / (sum of the chosen p); index[r][i] the expert.
+ * A logit of -inf has p = 0; a bias of -inf (or NaN) puts an expert behind all others.  Rows with nothing
+ * above -inf get weights of 0 under softmax and, where the sum is 0, when renormalised.  A row that holds a
+ * NaN (softmax: or +inf): weights NaN, index -1. */
+enum { PD_SCORE_SOFTMAX = 0, PD_SCORE_SIGMOID = 1 };
+enum { PD_GROUP_MAX = 0, PD_GROUP_TOP2 = 1 };
+int pd_route_experts(const void* logits, int dtype, int64_t rows, int64_t experts, int64_t row_stride,
+                     const float* bias, int score, int groups, int top_groups, int group_score, int top,
+                     int renormalise, float scale, float* weights, int32_t* index, void* stream);
+
+/* The gradient of the weights with respect to the logits (the choice itself has none), of their type, every
+ * expert of every row.  index: as returned, [rows][top]; entries outside 0..experts-1 are skipped, an expert
+ * named twice counts twice.  grad may be the logits themselves (same stride) or must not overlap them. */
+int pd_route_experts_grad(const void* logits, int dtype, int64_t rows, int64_t experts, int64_t row_stride,
+                          const int32_t* index, const float* grad_weights, int score, int top, int renormalise,
+                          float scale, void* grad, int64_t grad_stride, void* stream);
+
 /* ---- test hook (host only, touches no GPU) ----
  * The linear operator the sparse multi-scale peak stage evaluates for one axis of one scale --
  * scipy's Gaussian (sigma 3, reflect) after the second cubic resize (crop -> L outputs, predict.py:65)

@@ -14,7 +14,9 @@ LIB_PATH = os.environ.get('PD_LIBRARY') or os.path.join(_HERE, 'libposedecode.so
 PD_OK, PD_E_INVALID, PD_E_HIP, PD_E_OVERFLOW, PD_E_INDEX, PD_E_STATE = 0, -1, -2, -3, -4, -5
 MODE_P, MODE_D = 0, 1
 MEM_HOST, MEM_DEVICE = 0, 1
-F32, F64, U8 = 0, 1, 2
+F32, F64, U8, BF16, F16 = 0, 1, 2, 3, 4
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
+GROUP_MAX, GROUP_TOP2 = 0, 1
 IMPL_FAST, IMPL_SIMPLE, IMPL_STREAM = 0, 1, 2
 
 EXPORTS = ['pd_create', 'pd_destroy', 'pd_last_error', 'pd_version', 'pd_set_mode', 'pd_set_impl',
@@ -23,7 +25,8 @@ EXPORTS = ['pd_create', 'pd_destroy', 'pd_last_error', 'pd_version', 'pd_set_mod
            'pd_decode_batch', 'pd_decode_fullres', 'pd_pack', 'pd_sync_totals', 'pd_fetch',
            'pd_debug_smoothed', 'pd_packed_device', 'pd_profile', 'pd_profile_read', 'pd_results_host', 'pd_filter_stats', 'pd_profile_stages', 'pd_set_skeleton_buffer', 'pd_submit', 'pd_flush', 'pd_set_graph_replay', 'pd_set_host_results',
            'pd_decode_batch_static', 'pd_coco_rows', 'pd_image_resize_shape', 'pd_image_resize_pad', 'pd_render',
-           'pd_debug_found', 'pd_test_ms_axis', 'pd_comm_unique_id', 'pd_comm_create', 'pd_comm_destroy', 'pd_comm_last_error', 'pd_gather', 'pd_copy_used_skeletons']
+           'pd_debug_found', 'pd_test_ms_axis', 'pd_comm_unique_id', 'pd_comm_create', 'pd_comm_destroy', 'pd_comm_last_error', 'pd_gather', 'pd_copy_used_skeletons',
+           'pd_token_logprobs_workspace', 'pd_token_logprobs', 'pd_token_logprobs_grad', 'pd_route_experts', 'pd_route_experts_grad']
 
 STAGES = ['resize', 'smooth_nms', 'sort', 'pairs', 'match', 'parse', 'pack', 'filter', 'verify', 'planar', 'cells']
 
@@ -149,9 +152,16 @@ def lib():
     L.pd_comm_last_error.restype = C.c_char_p
     L.pd_gather.argtypes = [vp, C.POINTER(vp), i32, i32, vp, C.c_uint64, C.POINTER(C.c_uint64), C.POINTER(C.c_uint64)]
     L.pd_copy_used_skeletons.argtypes = [vp, vp, i32, C.c_uint64, vp]
+    i64, flt = C.c_int64, C.c_float
+    L.pd_token_logprobs_workspace.argtypes = [i32, i64, i64, i32]
+    L.pd_token_logprobs_workspace.restype = C.c_uint64
+    L.pd_token_logprobs.argtypes = [vp, i32, i64, i64, i64, vp, vp, i32, i32, vp, vp, vp, vp, vp, vp, C.c_uint64, vp]
+    L.pd_token_logprobs_grad.argtypes = [vp, i32, i64, i64, i64, vp, vp, vp, i32, vp, vp, vp, i64, vp]
+    L.pd_route_experts.argtypes = [vp, i32, i64, i64, i64, vp, i32, i32, i32, i32, i32, i32, flt, vp, vp, vp]
+    L.pd_route_experts_grad.argtypes = [vp, i32, i64, i64, i64, vp, vp, i32, i32, i32, flt, vp, i64, vp]
     for name in EXPORTS:
         fn = getattr(L, name)
-        if name not in ('pd_last_error', 'pd_version', 'pd_stream', 'pd_comm_last_error'):
+        if name not in ('pd_token_logprobs_workspace', 'pd_last_error', 'pd_version', 'pd_stream', 'pd_comm_last_error'):
             fn.restype = C.c_int
     _lib = L
     return L
