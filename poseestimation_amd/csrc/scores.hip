@@ -1,64 +1,241 @@
 // Operators on rows of scores: log probabilities of given tokens with entropy and top
 // alternatives, the routing of rows to experts, and the gradients of both.
-#include <hip/hip_bf16.h>
-#include <hip/hip_fp16.h>
+#include <type_traits>
 
 #include "common.h"
 
 #define SC_WG 256
+#define SC_WAVES (SC_WG / 64)
 #define SC_LOG2E 1.44269504088896340736f
 #define SC_LN2 0.69314718055994530942f
 
 // ---- elements ------------------------------------------------------------------------------
 
-__device__ __forceinline__ float sc_get(const float* p) { return *p; }
-__device__ __forceinline__ float sc_get(const __hip_bfloat16* p) {
-    return __uint_as_float((uint32_t)*(const uint16_t*)p << 16);
-}
-__device__ __forceinline__ float sc_get(const _Float16* p) { return (float)*p; }
+typedef uint32_t sc_u4 __attribute__((ext_vector_type(4)));
 
-__device__ __forceinline__ void sc_put(float* p, float v) { *p = v; }
-// round to nearest, ties to even; a NaN stays one
-__device__ __forceinline__ void sc_put(__hip_bfloat16* p, float v) {
-    const uint32_t u = __float_as_uint(v);
-    *(uint16_t*)p = (uint16_t)(v != v ? (u >> 16) | 0x40 : (u + 0x7fff + ((u >> 16) & 1)) >> 16);
-}
-__device__ __forceinline__ void sc_put(_Float16* p, float v) { *p = (_Float16)v; }
+// A type of the scores: V of them are 16 bytes, which is what a lane loads or stores at a time.  Rows start
+// wherever their stride puts them, so these accesses are aligned to the element only (the hardware takes
+// 16-byte accesses at any address).
+struct F32 {
+    typedef float E;
+    enum { V = 4 };
+    static __device__ __forceinline__ float get(const E* p) { return *p; }
+    static __device__ __forceinline__ void put(E* p, float v) { *p = v; }
+    static __device__ __forceinline__ void unpack(sc_u4 w, float* x) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(w[i]);
+    }
+    static __device__ __forceinline__ sc_u4 pack(const float* x) {
+        sc_u4 w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(x[i]);
+        return w;
+    }
+};
+struct BF16 {
+    typedef uint16_t E;
+    enum { V = 8 };
+    static __device__ __forceinline__ float get(const E* p) { return __uint_as_float((uint32_t)*p << 16); }
+    // to nearest, ties to even; a NaN stays one
+    static __device__ __forceinline__ E bits(float v) { return __builtin_bit_cast(uint16_t, (__bf16)v); }
+    static __device__ __forceinline__ void put(E* p, float v) { *p = bits(v); }
+    static __device__ __forceinline__ void unpack(sc_u4 w, float* x) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[2 * i] = __uint_as_float(w[i] << 16);
+            x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    }
+    static __device__ __forceinline__ sc_u4 pack(const float* x) {
+        sc_u4 w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = bits(x[2 * i]) | (uint32_t)bits(x[2 * i + 1]) << 16;
+        return w;
+    }
+};
+struct F16 {
+    typedef _Float16 E;
+    enum { V = 8 };
+    static __device__ __forceinline__ float get(const E* p) { return (float)*p; }
+    static __device__ __forceinline__ void put(E* p, float v) { *p = (_Float16)v; }
+    static __device__ __forceinline__ void unpack(sc_u4 w, float* x) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[2 * i] = (float)__builtin_bit_cast(_Float16, (uint16_t)w[i]);
+            x[2 * i + 1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[i] >> 16));
+        }
+    }
+    static __device__ __forceinline__ sc_u4 pack(const float* x) {
+        sc_u4 w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            w[i] = __builtin_bit_cast(uint16_t, (_Float16)x[2 * i]) | (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)x[2 * i + 1]) << 16;
+        return w;
+    }
+};
 
-// One whole number per (score, place): larger for the larger score, then for the lower place.
-__device__ __forceinline__ uint64_t sc_key(float x, uint32_t at) {
+template <typename E>
+struct __attribute__((packed, aligned(sizeof(E)))) ScVec {
+    sc_u4 v;
+};
+
+template <typename X>
+__device__ __forceinline__ sc_u4 sc_load(const typename X::E* p) {
+    return ((const ScVec<typename X::E>*)p)->v;
+}
+template <typename X>
+__device__ __forceinline__ void sc_store(typename X::E* p, sc_u4 w) {
+    ((ScVec<typename X::E>*)p)->v = w;
+}
+
+// Columns at .. at + V - 1 of a row that ends before column n; what lies behind is not read and becomes -inf.
+template <typename X>
+__device__ __forceinline__ void sc_read(const typename X::E* x, int at, int n, float* f) {
+    if (at + X::V <= n) {
+        X::unpack(sc_load<X>(x + at), f);
+    } else {
+#pragma unroll
+        for (int e = 0; e < X::V; ++e) f[e] = at + e < n ? X::get(x + at + e) : -INFINITY;
+    }
+}
+
+// One whole number per (score, place): larger for the larger score, then for the lower place.  No key is 0.
+__device__ __forceinline__ uint32_t sc_order(float x) {
     const uint32_t u = __float_as_uint(x + 0.0f);  // -0 counts as 0
-    const uint32_t o = (u >> 31) ? ~u : (u | 0x80000000u);
-    return ((uint64_t)o << 32) | (uint32_t)~at;
+    return (u >> 31) ? ~u : (u | 0x80000000u);
 }
-__device__ __forceinline__ float sc_key_score(uint64_t k) {
-    const uint32_t o = (uint32_t)(k >> 32);
-    return __uint_as_float((o >> 31) ? (o & 0x7fffffffu) : ~o);
-}
+__device__ __forceinline__ float sc_unorder(uint32_t o) { return __uint_as_float((o >> 31) ? (o & 0x7fffffffu) : ~o); }
+__device__ __forceinline__ uint64_t sc_key(float x, uint32_t at) { return ((uint64_t)sc_order(x) << 32) | (uint32_t)~at; }
+__device__ __forceinline__ float sc_key_score(uint64_t k) { return sc_unorder((uint32_t)(k >> 32)); }
 __device__ __forceinline__ uint32_t sc_key_place(uint64_t k) { return ~(uint32_t)k; }
 
-template <typename V, typename F>
-__device__ __forceinline__ V sc_wave(V v, F f) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) v = f(v, __shfl_xor(v, d));
-    return v;
-}
-struct SumOp { template <typename V> __device__ V operator()(V a, V b) const { return a + b; } };
-struct MaxOp { template <typename V> __device__ V operator()(V a, V b) const { return a > b ? a : b; } };
+// ---- reductions ----------------------------------------------------------------------------
 
-template <typename V, typename F>
-__device__ V sc_block(V v, F f, V* lds) {  // lds: SC_WG / 64 values
+struct SumOp { template <typename T> __device__ T operator()(T a, T b) const { return a + b; } };
+struct MaxOp { template <typename T> __device__ T operator()(T a, T b) const { return a > b ? a : b; } };
+struct FMaxOp { __device__ float operator()(float a, float b) const { return fmaxf(a, b); } };
+struct MinOp { template <typename T> __device__ T operator()(T a, T b) const { return a < b ? a : b; } };
+
+template <int CTRL>
+__device__ __forceinline__ uint32_t sc_dpp(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
+}
+
+// v of the lane STEP away in a butterfly; once the lanes of a group of STEP hold the same value any lane of the
+// neighbouring group will do, which is what lets the row mirrors stand in for the exchanges at 4 and 8.
+template <int STEP>
+__device__ __forceinline__ uint32_t sc_across(uint32_t v) {
+    if (STEP == 1) return sc_dpp<0xB1>(v);   // quad_perm 1 0 3 2
+    if (STEP == 2) return sc_dpp<0x4E>(v);   // quad_perm 2 3 0 1
+    if (STEP == 4) return sc_dpp<0x141>(v);  // row_half_mirror
+    if (STEP == 8) return sc_dpp<0x140>(v);  // row_mirror
+    return (uint32_t)__shfl_xor((int)v, STEP);
+}
+template <int STEP>
+__device__ __forceinline__ float sc_across(float v) { return __uint_as_float(sc_across<STEP>(__float_as_uint(v))); }
+template <int STEP>
+__device__ __forceinline__ double sc_across(double v) {
+    const uint64_t u = __double_as_longlong(v);
+    return __longlong_as_double((uint64_t)sc_across<STEP>((uint32_t)(u >> 32)) << 32 | sc_across<STEP>((uint32_t)u));
+}
+template <int STEP>
+__device__ __forceinline__ uint64_t sc_across(uint64_t u) {
+    return (uint64_t)sc_across<STEP>((uint32_t)(u >> 32)) << 32 | sc_across<STEP>((uint32_t)u);
+}
+
+// Over a whole wavefront, every lane taking part; all get the result.
+template <typename T, typename F>
+__device__ __forceinline__ T sc_wave(T v, F f) {
+    v = f(v, sc_across<1>(v));
+    v = f(v, sc_across<2>(v));
+    v = f(v, sc_across<4>(v));
+    v = f(v, sc_across<8>(v));
+    v = f(v, sc_across<16>(v));
+    return f(v, sc_across<32>(v));
+}
+
+template <typename T, typename F>
+__device__ T sc_block(T v, F f, T* lds) {  // lds: SC_WAVES values
     v = sc_wave(v, f);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
     __syncthreads();
     v = lds[0];
 #pragma unroll
-    for (int i = 1; i < SC_WG / 64; ++i) v = f(v, lds[i]);
+    for (int i = 1; i < SC_WAVES; ++i) v = f(v, lds[i]);
     return v;
 }
 
 // ---- log probabilities ---------------------------------------------------------------------
+//
+// One pass over the row.  A lane keeps the largest score m it has seen, S = sum 2^t and W = sum 2^t t with
+// t = (x - m) log2 e, and takes a chunk of scores at a time: the chunk's maximum first, then S and W are carried
+// to it (S' = 2^d S, W' = 2^d (W + S d), d the step of m in the same units), then the chunk is added.  Lanes,
+// wavefronts and slices of a row are joined by the same rule.  log S and the entropy log S - ln 2 W / S follow,
+// both sums of terms of one sign.  The statistics are float32; a lane adds n / 64 (a wavefront to the row) or
+// n / 256 terms one by one.
+//
+// The alternatives need no second look at the row either: the K-th largest of the lanes' maxima, tau, is a lower
+// bound of the K-th largest score, so that only the few segments (a lane's part of a chunk) whose maximum reaches
+// tau are read again, and only their scores that reach it are put into order.
+
+struct Stat {
+    float m, s, w;
+};
+
+// 2^-256 is 0 in float32: below that t only has to stay finite, 0 * -inf being no number.
+__device__ __forceinline__ float sc_floor_t(float t) { return fmaxf(t, -256.0f); }
+
+// st carried to the maximum `to` >= st.m.
+__device__ __forceinline__ void sc_carry(Stat& st, float to) {
+    const float base = to == -INFINITY ? 0.0f : to;
+    const float d = sc_floor_t((st.m - base) * SC_LOG2E), f = __builtin_amdgcn_exp2f(d);
+    st.w = f * fmaf(st.s, d, st.w);
+    st.s *= f;
+    st.m = to;
+}
+
+template <int N>
+__device__ __forceinline__ float sc_max(const float* x, float m) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) m = fmaxf(m, x[i]);
+    return m;
+}
+
+template <int N>
+__device__ __forceinline__ void sc_add(Stat& st, const float* x) {
+    const float base = st.m == -INFINITY ? 0.0f : st.m;
+    float s[2] = {0, 0}, w[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float t = (x[i] - base) * SC_LOG2E, e = __builtin_amdgcn_exp2f(t);
+        s[i & 1] += e;  // a NaN, or +inf, shows up here
+        w[i & 1] = fmaf(e, sc_floor_t(t), w[i & 1]);
+    }
+    st.s += s[0] + s[1];
+    st.w += w[0] + w[1];
+}
+
+__device__ __forceinline__ void sc_join_wave(Stat& st) {
+    sc_carry(st, sc_wave(st.m, FMaxOp()));
+    st.s = sc_wave(st.s, SumOp());
+    st.w = sc_wave(st.w, SumOp());
+}
+
+struct RowStat {
+    float base, log_sum, entropy;  // base: the largest score, 0 for an empty row
+    bool empty, bad;               // nothing above -inf; a NaN or +inf among the scores
+};
+
+__device__ __forceinline__ RowStat sc_row_stat(const Stat& st) {
+    RowStat q;
+    q.empty = st.s == 0;
+    q.bad = st.s != st.s;
+    q.base = st.m == -INFINITY ? 0.0f : st.m;
+    q.log_sum = q.empty ? 0.0f : logf(st.s);
+    q.entropy = q.empty ? 0.0f : q.log_sum - SC_LN2 * st.w / st.s;
+    return q;
+}
 
 struct LogprobArgs {
     const void* x;
@@ -69,62 +246,422 @@ struct LogprobArgs {
     int n_tok, top;
     float *logp, *entropy, *stats, *top_logp;
     int32_t* top_index;
+    int slices, slice_cols;  // a row in parts, one workgroup each (slice_cols a multiple of SC_CHUNK)
+    Stat* part;              // [rows][slices]
+    uint64_t* part_keys;     // [rows][slices][top], 0: none
 };
 
 __device__ __forceinline__ int sc_width(const int32_t* widths, int64_t r, int cols) {
     return widths ? pd_clampi(widths[r], 0, cols) : cols;
 }
 
+// Statistics and token log probabilities of row r, by threads i = 0 .. count - 1.
 template <typename X>
-__global__ __launch_bounds__(SC_WG) void k_token_logprobs(LogprobArgs a) {
-    __shared__ float lf[SC_WG / 64];
-    __shared__ uint64_t lk[SC_WG / 64];
-    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
-        const X* x = (const X*)a.x + r * a.stride;
+__device__ __forceinline__ void sc_put_row(const LogprobArgs& a, int64_t r, const typename X::E* x, int n, const Stat& st,
+                                           const RowStat& q, int i, int count) {
+    if (i == 0) {
+        if (a.stats) {
+            a.stats[3 * r] = st.m;
+            a.stats[3 * r + 1] = q.log_sum;
+            a.stats[3 * r + 2] = q.entropy;
+        }
+        if (a.entropy) a.entropy[r] = q.entropy;
+    }
+    for (int t = i; t < a.n_tok; t += count) {
+        const int64_t tok = a.tokens[r * a.n_tok + t];
+        float v = 0;
+        if (tok >= 0) v = q.empty ? -INFINITY : ((tok < n ? X::get(x + tok) : -INFINITY) - q.base) - q.log_sum;
+        a.logp[r * a.n_tok + t] = v;
+    }
+}
+
+// Alternative k of row r; key 0: the row has no more scores, what lies behind it counts as -inf.
+__device__ __forceinline__ void sc_put_top(const LogprobArgs& a, int64_t r, int k, uint64_t key, const RowStat& q) {
+    const int64_t at = r * a.top + k;
+    a.top_index[at] = q.bad ? -1 : key ? (int)sc_key_place(key) : k;
+    a.top_logp[at] = q.bad ? NAN : q.empty || !key ? -INFINITY : (sc_key_score(key) - q.base) - q.log_sum;
+}
+
+// The K-th largest of the orders o[0 .. N-1] of a wavefront's lanes, by its bits from the top; as soon as exactly K
+// values lie above the bits so far it is the least of them.
+template <int N>
+__device__ __forceinline__ uint32_t sc_kth(const uint32_t* o, int K) {
+    uint32_t t = 0;
+    for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t trial = t | 1u << bit;
+        int count = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) count += __popcll(__ballot(o[i] >= trial));
+        if (count >= K) t = trial;
+        if (count == K) {
+            uint32_t least = ~0u;
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (o[i] >= trial && o[i] < least) least = o[i];
+            return sc_wave(least, MinOp());
+        }
+    }
+    return t;
+}
+
+// ---- a wavefront to the row: up to 2048 columns, all of them in registers ---------------------
+//
+// Bound by instruction issue, not by memory: a row of a few hundred columns is some ten instructions a score and
+// as many again a row for the reductions and the alternatives, so nothing is exchanged through LDS but the handful
+// of candidates, and wavefronts do not wait for each other.
+
+#define SC_WAVE_CAND 128  // candidates of a row; more (equal scores) are found one by one
+
+template <typename X, int NV>
+__global__ __launch_bounds__(SC_WG) void k_token_logprobs_wave(LogprobArgs a) {
+    constexpr int V = X::V, N = NV * V;
+    __shared__ uint64_t cand[SC_WAVES][SC_WAVE_CAND];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint64_t* mine = cand[wave];
+    for (int64_t r = (int64_t)blockIdx.x * SC_WAVES + wave; r < a.rows; r += (int64_t)gridDim.x * SC_WAVES) {
+        const typename X::E* x = (const typename X::E*)a.x + r * a.stride;
         const int n = sc_width(a.widths, r, a.cols);
-        float m = -INFINITY;
-        for (int j = threadIdx.x; j < n; j += SC_WG) m = fmaxf(m, sc_get(x + j));
-        m = sc_block(m, MaxOp(), lf);
-        const float mb = m == -INFINITY ? 0.0f : m;
-        float s = 0, w = 0;
-        for (int j = threadIdx.x; j < n; j += SC_WG) {
-            const float t = (sc_get(x + j) - mb) * SC_LOG2E, e = exp2f(t);
-            s += e;
-            w = fmaf(e, fmaxf(t, -256.0f), w);
+        float f[N];
+#pragma unroll
+        for (int u = 0; u < NV; ++u) sc_read<X>(x, (u * 64 + lane) * V, n, f + u * V);
+        const float m = sc_max<N>(f, -INFINITY);
+        Stat st = {sc_wave(m, FMaxOp()), 0, 0};
+        sc_add<N>(st, f);
+        st.s = sc_wave(st.s, SumOp());
+        st.w = sc_wave(st.w, SumOp());
+        const RowStat q = sc_row_stat(st);
+        sc_put_row<X>(a, r, x, n, st, q, lane, 64);
+        if (!a.top) continue;
+        if (q.bad || q.empty) {
+            if (lane < a.top) sc_put_top(a, r, lane, q.bad ? 0 : sc_key(-INFINITY, lane), q);
+            continue;
         }
-        s = sc_block(s, SumOp(), lf);
-        w = sc_block(w, SumOp(), lf);
-        const bool empty = s == 0, bad = s != s;
-        const float log_sum = empty ? 0.0f : logf(s), h = empty ? 0.0f : log_sum - SC_LN2 * w / s;
-        if (threadIdx.x == 0) {
-            if (a.stats) {
-                a.stats[3 * r] = m;
-                a.stats[3 * r + 1] = log_sum;
-                a.stats[3 * r + 2] = h;
+        const uint32_t mo = sc_order(m);
+        const float tau = sc_unorder(sc_kth<1>(&mo, a.top));
+        int count = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int at = ((i / V) * 64 + lane) * V + i % V;
+            const bool in = f[i] >= tau && at < n;
+            const uint64_t mask = __ballot(in);
+            if (mask) {
+                const int to = count + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+                if (in && to < SC_WAVE_CAND) mine[to] = sc_key(f[i], at);
+                count += __popcll(mask);
             }
-            if (a.entropy) a.entropy[r] = h;
         }
-        for (int t = threadIdx.x; t < a.n_tok; t += SC_WG) {
-            const int64_t tok = a.tokens[r * a.n_tok + t];
-            float v = 0;
-            if (tok >= 0) v = empty ? -INFINITY : ((tok < n ? sc_get(x + tok) : -INFINITY) - mb) - log_sum;
-            a.logp[r * a.n_tok + t] = v;
-        }
-        uint64_t prev = ~0ull;
-        for (int k = 0; k < a.top; ++k) {
-            uint64_t best = 0;
-            if (!bad && !empty)
-                for (int j = threadIdx.x; j < n; j += SC_WG) {
-                    const uint64_t key = sc_key(sc_get(x + j), j);
-                    if (key < prev && key > best) best = key;
+        pd_wave_sync();
+        if (count <= SC_WAVE_CAND) {
+            for (int i = lane; i < count; i += 64) {
+                const uint64_t key = mine[i];
+                int rank = 0;
+                for (int j = 0; j < count; ++j) rank += mine[j] > key;
+                if (rank < a.top) sc_put_top(a, r, rank, key, q);
+            }
+            if (lane >= count && lane < a.top) sc_put_top(a, r, lane, 0, q);
+        } else {
+            uint64_t prev = ~0ull;
+            for (int k = 0; k < a.top; ++k) {
+                uint64_t best = 0;
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const int at = ((i / V) * 64 + lane) * V + i % V;
+                    const uint64_t key = sc_key(f[i], at);
+                    if (at < n && key < prev && key > best) best = key;
                 }
-            best = sc_block(best, MaxOp(), lk);
-            prev = best;
-            if (threadIdx.x == 0) {
-                a.top_index[r * a.top + k] = bad ? -1 : best ? (int)sc_key_place(best) : k;
-                a.top_logp[r * a.top + k] = bad ? NAN : best ? (sc_key_score(best) - mb) - log_sum : -INFINITY;
+                prev = sc_wave(best, MaxOp());
+                if (lane == 0) sc_put_top(a, r, k, prev, q);
             }
         }
+        pd_wave_sync();  // the next row's candidates go to the same place
+    }
+}
+
+// ---- a workgroup to the row, or to a slice of it ------------------------------------------------
+//
+// Chunks of 8192 columns, 32 to a thread in 16-byte loads; eight workgroups to a CU keep the loads coming while
+// others reduce.  Bound by the memory where there are rows enough.  A row is cut into slices of whole chunks where
+// rows alone do not fill the chip, or where it is longer than SC_MAX_CHUNKS chunks; the slices are joined by
+// k_token_logprobs_join.
+
+#define SC_PER_THREAD 32
+#define SC_CHUNK (SC_WG * SC_PER_THREAD)
+#define SC_MAX_CHUNKS 16
+#define SC_SEGS 128   // segments that are read again
+#define SC_CAND 512   // candidates that are put into order
+
+struct TopShared {
+    uint32_t seg_max[SC_MAX_CHUNKS][SC_WG];
+    uint32_t lane_max[SC_WG];
+    uint64_t cand[SC_CAND];
+    uint64_t wave_best[SC_WAVES];
+    uint16_t segs[SC_SEGS];
+    uint32_t tau;
+    int n_seg, n_cand, scanned[SC_WAVES];
+};
+
+// Reads the segments whose maximum is at least `from` again and collects their scores from there on (orders).
+// False: there are more of either than there is room for.
+template <typename X>
+__device__ bool sc_collect(TopShared& sh, const typename X::E* x, int begin, int end, uint32_t from) {
+    constexpr int V = X::V, NV = SC_PER_THREAD / V;
+    const int t = threadIdx.x;
+    __syncthreads();
+    if (t == 0) sh.n_seg = sh.n_cand = 0;
+    __syncthreads();
+    const int chunks = (end - begin + SC_CHUNK - 1) / SC_CHUNK;
+    for (int c = 0; c < chunks; ++c)
+        if (sh.seg_max[c][t] >= from) {
+            const int to = atomicAdd(&sh.n_seg, 1);
+            if (to < SC_SEGS) sh.segs[to] = (uint16_t)(c * SC_WG + t);
+        }
+    __syncthreads();
+    if (sh.n_seg > SC_SEGS) return false;
+    for (int i = t; i < sh.n_seg * NV; i += SC_WG) {
+        const int seg = sh.segs[i / NV];
+        const int at = begin + (seg / SC_WG) * SC_CHUNK + ((i % NV) * SC_WG + seg % SC_WG) * V;
+        if (at >= end) continue;
+        float f[V];
+        sc_read<X>(x, at, end, f);
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+            if (sc_order(f[e]) >= from && at + e < end) {
+                const int to = atomicAdd(&sh.n_cand, 1);
+                if (to < SC_CAND) sh.cand[to] = sc_key(f[e], at + e);
+            }
+    }
+    __syncthreads();
+    return sh.n_cand <= SC_CAND;
+}
+
+// The `top` largest of columns begin .. end - 1 as keys, put(k, key) called once for each k, with 0 where there
+// are no more columns.  lane_max: the largest of this thread's columns.  The segments' maxima are in sh.
+template <typename X, typename Put>
+__device__ void sc_top_block(TopShared& sh, const typename X::E* x, int begin, int end, int top, float lane_max, Put put) {
+    constexpr int V = X::V;
+    const int t = threadIdx.x;
+    sh.lane_max[t] = sc_order(lane_max);
+    __syncthreads();
+    if (t < 64) {
+        uint32_t o[SC_WAVES];
+#pragma unroll
+        for (int i = 0; i < SC_WAVES; ++i) o[i] = sh.lane_max[t + 64 * i];
+        const uint32_t tau = sc_kth<SC_WAVES>(o, top);
+        if (t == 0) sh.tau = tau;
+    }
+    __syncthreads();
+    const uint32_t tau = sh.tau;
+    bool fits = sc_collect<X>(sh, x, begin, end, tau);
+    if (!fits && sc_collect<X>(sh, x, begin, end, tau + 1)) {
+        // too many scores equal to tau (a masked row, a constant one): what is larger has been collected, and the
+        // first of the equal ones make up the number, found from the front
+        fits = true;
+        for (int at0 = begin; at0 < end && sh.n_cand < top; at0 += SC_WG * V) {
+            const int at = at0 + t * V;
+            float f[V];
+            sc_read<X>(x, at, end, f);
+            int mine = 0;
+#pragma unroll
+            for (int e = 0; e < V; ++e) mine += at + e < end && sc_order(f[e]) == tau;
+            int before = mine;  // an inclusive scan over the wavefront
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const int o = __shfl_up(before, d);
+                if ((t & 63) >= d) before += o;
+            }
+            if ((t & 63) == 63) sh.scanned[t >> 6] = before;
+            const int have = sh.n_cand;
+            __syncthreads();
+            int total = 0;
+            before += have - mine;
+#pragma unroll
+            for (int i = 0; i < SC_WAVES; ++i) {
+                if (i < t >> 6) before += sh.scanned[i];
+                total += sh.scanned[i];
+            }
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                if (at + e < end && sc_order(f[e]) == tau) {
+                    if (before < top) sh.cand[before] = sc_key(f[e], at + e);
+                    ++before;
+                }
+            if (t == 0) sh.n_cand = have + total < top ? have + total : top;
+            __syncthreads();
+        }
+    }
+    if (fits) {
+        const int n = sh.n_cand;
+        for (int i = t; i < n; i += SC_WG) {
+            const uint64_t key = sh.cand[i];
+            int rank = 0;
+            for (int j = 0; j < n; ++j) rank += sh.cand[j] > key;
+            if (rank < top) put(rank, key);
+        }
+        if (t >= n && t < top) put(t, 0);
+    } else {
+        uint64_t prev = ~0ull;  // many large scores in few lanes: one after the other
+        for (int k = 0; k < top; ++k) {
+            uint64_t best = 0;
+            for (int at = begin + t * V; at < end; at += SC_WG * V) {
+                float f[V];
+                sc_read<X>(x, at, end, f);
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    const uint64_t key = sc_key(f[e], at + e);
+                    if (at + e < end && key < prev && key > best) best = key;
+                }
+            }
+            prev = sc_block(best, MaxOp(), sh.wave_best);
+            if (t == 0) put(k, prev);
+        }
+    }
+    __syncthreads();
+}
+
+struct Nothing {};
+
+template <typename X, bool TOP>
+__global__ __launch_bounds__(SC_WG) void k_token_logprobs_block(LogprobArgs a) {
+    constexpr int V = X::V, NV = SC_PER_THREAD / V;
+    __shared__ Stat wave_stat[SC_WAVES];
+    __shared__ typename std::conditional<TOP, TopShared, Nothing>::type sh;
+    const int t = threadIdx.x;
+    for (int64_t b = blockIdx.x; b < a.rows * a.slices; b += gridDim.x) {
+        const int64_t r = b / a.slices;
+        const int slice = (int)(b - r * a.slices);
+        const typename X::E* x = (const typename X::E*)a.x + r * a.stride;
+        const int n = sc_width(a.widths, r, a.cols);
+        const int begin = slice * a.slice_cols < n ? slice * a.slice_cols : n;
+        const int end = n - begin < a.slice_cols ? n : begin + a.slice_cols;
+        Stat st = {-INFINITY, 0, 0};
+        for (int c = 0, at0 = begin; at0 < end; at0 += SC_CHUNK, ++c) {
+            float f[SC_PER_THREAD];
+            if (at0 + SC_CHUNK <= end) {
+                sc_u4 w[NV];
+#pragma unroll
+                for (int u = 0; u < NV; ++u) w[u] = sc_load<X>(x + at0 + (u * SC_WG + t) * V);
+#pragma unroll
+                for (int u = 0; u < NV; ++u) X::unpack(w[u], f + u * V);
+            } else {
+#pragma unroll
+                for (int u = 0; u < NV; ++u) sc_read<X>(x, at0 + (u * SC_WG + t) * V, end, f + u * V);
+            }
+            const float m = sc_max<SC_PER_THREAD>(f, -INFINITY);
+            if constexpr (TOP) sh.seg_max[c][t] = sc_order(m);
+            sc_carry(st, fmaxf(st.m, m));
+            sc_add<SC_PER_THREAD>(st, f);
+        }
+        const float lane_max = st.m;
+        sc_join_wave(st);
+        if ((t & 63) == 0) wave_stat[t >> 6] = st;
+        __syncthreads();
+        st = wave_stat[0];
+#pragma unroll
+        for (int i = 1; i < SC_WAVES; ++i) {
+            Stat o = wave_stat[i];
+            const float m = fmaxf(st.m, o.m);
+            sc_carry(st, m);
+            sc_carry(o, m);
+            st.s += o.s;
+            st.w += o.w;
+        }
+        const RowStat q = sc_row_stat(st);
+        if (a.slices > 1) {
+            if (t == 0) a.part[b] = st;
+        } else {
+            sc_put_row<X>(a, r, x, n, st, q, t, SC_WG);
+        }
+        if constexpr (TOP) {
+            if (a.slices > 1) {
+                uint64_t* keys = a.part_keys + b * a.top;
+                if (q.bad) {
+                    if (t < a.top) keys[t] = 0;
+                } else {
+                    sc_top_block<X>(sh, x, begin, end, a.top, lane_max, [&](int k, uint64_t key) { keys[k] = key; });
+                }
+            } else if (q.bad || q.empty) {
+                if (t < a.top) sc_put_top(a, r, t, q.bad ? 0 : sc_key(-INFINITY, t), q);
+            } else {
+                sc_top_block<X>(sh, x, begin, end, a.top, lane_max, [&](int k, uint64_t key) { sc_put_top(a, r, k, key, q); });
+            }
+        }
+        __syncthreads();  // wave_stat is written again
+    }
+}
+
+// The slices of a row: their statistics by the rule above, their alternatives (each slice's in order) merged.  With
+// j = ceil(top / slices) the least of the slices' j-th keys has at least `top` keys from it on.
+template <typename X>
+__global__ __launch_bounds__(SC_WG) void k_token_logprobs_join(LogprobArgs a) {
+    __shared__ uint64_t cand[SC_CAND], wave_key[SC_WAVES];
+    __shared__ Stat wave_stat[SC_WAVES];
+    __shared__ int n_cand;
+    const int t = threadIdx.x;
+    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+        const typename X::E* x = (const typename X::E*)a.x + r * a.stride;
+        const int n = sc_width(a.widths, r, a.cols);
+        Stat st = {-INFINITY, 0, 0};
+        for (int i = t; i < a.slices; i += SC_WG) {
+            Stat o = a.part[r * a.slices + i];
+            const float m = fmaxf(st.m, o.m);
+            sc_carry(st, m);
+            sc_carry(o, m);
+            st.s += o.s;
+            st.w += o.w;
+        }
+        sc_join_wave(st);
+        if (t == 0) n_cand = 0;
+        if ((t & 63) == 0) wave_stat[t >> 6] = st;
+        __syncthreads();
+        st = wave_stat[0];
+#pragma unroll
+        for (int i = 1; i < SC_WAVES; ++i) {
+            Stat o = wave_stat[i];
+            const float m = fmaxf(st.m, o.m);
+            sc_carry(st, m);
+            sc_carry(o, m);
+            st.s += o.s;
+            st.w += o.w;
+        }
+        const RowStat q = sc_row_stat(st);
+        sc_put_row<X>(a, r, x, n, st, q, t, SC_WG);
+        if (a.top && (q.bad || q.empty)) {
+            if (t < a.top) sc_put_top(a, r, t, q.bad ? 0 : sc_key(-INFINITY, t), q);
+        } else if (a.top) {
+            const uint64_t* keys = a.part_keys + r * a.slices * a.top;
+            const int total = a.slices * a.top, j = (a.top + a.slices - 1) / a.slices;
+            uint64_t from = ~0ull;
+            for (int i = t; i < a.slices; i += SC_WG) from = MinOp()(from, keys[i * a.top + j - 1]);
+            from = sc_block(from, MinOp(), wave_key);
+            for (int i = t; i < total; i += SC_WG) {
+                const uint64_t key = keys[i];
+                if (key && key >= from) {
+                    const int to = atomicAdd(&n_cand, 1);
+                    if (to < SC_CAND) cand[to] = key;
+                }
+            }
+            __syncthreads();
+            const int have = n_cand;
+            if (have <= SC_CAND) {
+                for (int i = t; i < have; i += SC_WG) {
+                    const uint64_t key = cand[i];
+                    int rank = 0;
+                    for (int k = 0; k < have; ++k) rank += cand[k] > key;
+                    if (rank < a.top) sc_put_top(a, r, rank, key, q);
+                }
+                if (t >= have && t < a.top) sc_put_top(a, r, t, 0, q);
+            } else {
+                uint64_t prev = ~0ull;
+                for (int k = 0; k < a.top; ++k) {
+                    uint64_t best = 0;
+                    for (int i = t; i < total; i += SC_WG)
+                        if (keys[i] < prev && keys[i] > best) best = keys[i];
+                    prev = sc_block(best, MaxOp(), wave_key);
+                    if (t == 0) sc_put_top(a, r, k, prev, q);
+                }
+            }
+        }
+        __syncthreads();
     }
 }
 
@@ -144,8 +681,8 @@ struct LogprobGradArgs {
 template <typename X>
 __global__ __launch_bounds__(SC_WG) void k_token_logprobs_grad(LogprobGradArgs a) {
     for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
-        const X* x = (const X*)a.x + r * a.stride;
-        X* out = (X*)a.out + r * a.out_stride;
+        const typename X::E* x = (const typename X::E*)a.x + r * a.stride;
+        typename X::E* out = (typename X::E*)a.out + r * a.out_stride;
         const int n = sc_width(a.widths, r, a.cols);
         const float m = a.stats[3 * r], log_sum = a.stats[3 * r + 1], h = a.stats[3 * r + 2];
         const bool empty = m == -INFINITY && log_sum == 0;
@@ -156,12 +693,12 @@ __global__ __launch_bounds__(SC_WG) void k_token_logprobs_grad(LogprobGradArgs a
         for (int j = threadIdx.x; j < a.cols; j += SC_WG) {
             float d = 0;
             if (j < n && !empty) {
-                const float lp = (sc_get(x + j) - m) - log_sum, p = exp2f(lp * SC_LOG2E);
+                const float lp = (X::get(x + j) - m) - log_sum, p = exp2f(lp * SC_LOG2E);
                 d = -p * (g + ge * (fmaxf(lp, -256.0f) + h));
                 for (int t = 0; t < a.n_tok; ++t)
                     if (a.tokens[r * a.n_tok + t] == j) d += a.g_logp[r * a.n_tok + t];
             }
-            sc_put(out + j, d);
+            X::put(out + j, d);
         }
     }
 }
@@ -211,12 +748,12 @@ __device__ __forceinline__ void sc_route_weights(const RouteArgs& a, int64_t r, 
 // One row by one wavefront, the order decided in float64.
 template <typename X>
 __device__ void sc_route_row(const RouteArgs& a, int64_t r, int lane) {
-    const X* x = (const X*)a.x + r * a.stride;
+    const typename X::E* x = (const typename X::E*)a.x + r * a.stride;
     const int E = a.experts, per_group = E / a.groups;
     float m = -INFINITY;
     bool nan = false;
     for (int j = lane; j < E; j += 64) {
-        const float v = sc_get(x + j);
+        const float v = X::get(x + j);
         nan |= v != v || (v == INFINITY && !a.sigmoid);
         m = fmaxf(m, v);
     }
@@ -224,7 +761,7 @@ __device__ void sc_route_row(const RouteArgs& a, int64_t r, int lane) {
     m = sc_wave(m, MaxOp());
     double total = 0;
     if (!a.sigmoid && m > -INFINITY)
-        for (int j = lane; j < E; j += 64) total += exp((double)sc_get(x + j) - m);
+        for (int j = lane; j < E; j += 64) total += exp((double)X::get(x + j) - m);
     total = sc_wave(total, SumOp());
     double p[SC_PER_LANE], by[SC_PER_LANE];
 #pragma unroll
@@ -232,7 +769,7 @@ __device__ void sc_route_row(const RouteArgs& a, int64_t r, int lane) {
         const int j = lane + 64 * i;
         p[i] = by[i] = -INFINITY;
         if (j >= E) continue;
-        const double v = sc_get(x + j);
+        const double v = X::get(x + j);
         p[i] = a.sigmoid ? 1 / (1 + exp(-v)) : total > 0 ? exp(v - m) / total : 0.0;
         by[i] = a.bias ? p[i] + (double)a.bias[j] : v;
         if (!(by[i] >= -1e300)) by[i] = -1e300;  // -inf or NaN: behind every other, before what no group offers
@@ -290,7 +827,7 @@ __device__ void sc_route_row(const RouteArgs& a, int64_t r, int lane) {
         if (lane == k) chosen = at;
     }
     const int idx = nan ? -1 : chosen;
-    const float xi = lane < a.top && idx >= 0 ? sc_get(x + idx) : -INFINITY;
+    const float xi = lane < a.top && idx >= 0 ? X::get(x + idx) : -INFINITY;
     sc_route_weights(a, r, lane, idx, xi, m, (float)total);
 }
 
@@ -316,13 +853,13 @@ template <typename X>
 __global__ __launch_bounds__(SC_WG) void k_route_grad(RouteGradArgs a) {
     const int lane = threadIdx.x & 63;
     for (int64_t r = (int64_t)blockIdx.x * (SC_WG / 64) + (threadIdx.x >> 6); r < a.rows; r += (int64_t)gridDim.x * (SC_WG / 64)) {
-        const X* x = (const X*)a.x + r * a.stride;
-        X* out = (X*)a.out + r * a.out_stride;
+        const typename X::E* x = (const typename X::E*)a.x + r * a.stride;
+        typename X::E* out = (typename X::E*)a.out + r * a.out_stride;
         const int E = a.experts;
         const int idx = lane < a.top ? a.index[r * a.top + lane] : -1;
         const bool have = idx >= 0 && idx < E;
         const float g = have ? a.g[r * a.top + lane] * a.scale : 0.0f;
-        const float xi = have ? sc_get(x + idx) : -INFINITY;
+        const float xi = have ? X::get(x + idx) : -INFINITY;
         const bool dense = !a.sigmoid && !a.renorm;
         float m = 0, total = 0, wgt, c;
         if (a.sigmoid || a.renorm) {
@@ -344,10 +881,10 @@ __global__ __launch_bounds__(SC_WG) void k_route_grad(RouteGradArgs a) {
             if (a.sigmoid) c *= xi > 0 ? expf(-xi) / (1 + expf(-xi)) : 1 / (1 + expf(xi));  // 1 - p
         } else {
             m = -INFINITY;
-            for (int j = lane; j < E; j += 64) m = fmaxf(m, sc_get(x + j));
+            for (int j = lane; j < E; j += 64) m = fmaxf(m, X::get(x + j));
             m = sc_wave(m, MaxOp());
             if (m > -INFINITY)
-                for (int j = lane; j < E; j += 64) total += expf(sc_get(x + j) - m);
+                for (int j = lane; j < E; j += 64) total += expf(X::get(x + j) - m);
             total = sc_wave(total, SumOp());
             wgt = have && total != 0 ? expf(xi - m) / total : 0.0f;
             c = wgt * g;
@@ -356,13 +893,13 @@ __global__ __launch_bounds__(SC_WG) void k_route_grad(RouteGradArgs a) {
         for (int j0 = 0; j0 < E; j0 += 64) {
             const int j = j0 + lane;
             float d = 0;
-            if (dense && j < E && total != 0) d = -(expf(sc_get(x + j) - m) / total) * all;
+            if (dense && j < E && total != 0) d = -(expf(X::get(x + j) - m) / total) * all;
             for (int k = 0; k < a.top; ++k) {
                 const int at = __shfl(have ? idx : -1, k);
                 const float v = __shfl(c, k);
                 if (at == j) d += v;
             }
-            if (j < E) sc_put(out + j, d);
+            if (j < E) X::put(out + j, d);
         }
     }
 }
@@ -381,9 +918,10 @@ static int sc_launched(const char* fn) {
     return PD_E_HIP;
 }
 
-static int sc_size(int dtype) { return dtype == PD_F32 ? 4 : dtype == PD_BF16 || dtype == PD_F16 ? 2 : 0; }
-
+// Rows beyond this many workgroups are taken in turns.
 static unsigned sc_grid(int64_t wanted) { return (unsigned)(wanted < 1 << 20 ? wanted : 1 << 20); }
+
+static int sc_size(int dtype) { return dtype == PD_F32 ? 4 : dtype == PD_BF16 || dtype == PD_F16 ? 2 : 0; }
 
 // What the calls have in common; 1: nothing to do.
 static int sc_check_rows(const char* fn, const void* x, int dtype, int64_t rows, int64_t cols, int64_t stride, int64_t max_cols) {
@@ -415,14 +953,62 @@ static int sc_check_grad(const char* fn, const void* x, int dtype, int64_t rows,
 #define SC_BY_TYPE(dtype, kernel, grid, stream, args)                                                          \
     do {                                                                                                       \
         if ((dtype) == PD_F32)                                                                                 \
-            hipLaunchKernelGGL((kernel<float>), dim3(grid), dim3(SC_WG), 0, (hipStream_t)(stream), args);      \
+            hipLaunchKernelGGL((kernel<F32>), dim3(grid), dim3(SC_WG), 0, (hipStream_t)(stream), args);      \
         else if ((dtype) == PD_BF16)                                                                           \
-            hipLaunchKernelGGL((kernel<__hip_bfloat16>), dim3(grid), dim3(SC_WG), 0, (hipStream_t)(stream), args); \
+            hipLaunchKernelGGL((kernel<BF16>), dim3(grid), dim3(SC_WG), 0, (hipStream_t)(stream), args); \
         else                                                                                                   \
-            hipLaunchKernelGGL((kernel<_Float16>), dim3(grid), dim3(SC_WG), 0, (hipStream_t)(stream), args);   \
+            hipLaunchKernelGGL((kernel<F16>), dim3(grid), dim3(SC_WG), 0, (hipStream_t)(stream), args);   \
     } while (0)
 
-extern "C" uint64_t pd_token_logprobs_workspace(int dtype, int64_t rows, int64_t columns, int top) { return 0; }
+// How a call with a workgroup to the row is cut.  The chip runs some 2000 workgroups at a time; with fewer rows than
+// SC_FILL a row is cut into more slices, of whole chunks.
+#define SC_WAVE_COLS 2048
+#define SC_FILL 512
+
+static void sc_slices(int64_t rows, int64_t cols, int* slices, int* slice_cols) {
+    const int64_t chunks = (cols + SC_CHUNK - 1) / SC_CHUNK;
+    int64_t want = rows >= SC_FILL ? 1 : SC_FILL / rows;
+    const int64_t least = (chunks + SC_MAX_CHUNKS - 1) / SC_MAX_CHUNKS;
+    if (want < least) want = least;
+    if (want > chunks) want = chunks;
+    const int64_t each = (chunks + want - 1) / want;
+    *slices = (int)((chunks + each - 1) / each);
+    *slice_cols = (int)each * SC_CHUNK;
+}
+
+extern "C" uint64_t pd_token_logprobs_workspace(int dtype, int64_t rows, int64_t columns, int top) {
+    if (!sc_size(dtype) || rows < 1 || rows > INT32_MAX || columns <= SC_WAVE_COLS || columns > PD_MAX_COLUMNS || top < 0 ||
+        top > PD_MAX_ALTERNATIVES)
+        return 0;
+    int slices, slice_cols;
+    sc_slices(rows, columns, &slices, &slice_cols);
+    if (slices == 1) return 0;
+    return (((uint64_t)rows * slices * sizeof(Stat) + 15) & ~15ull) + (uint64_t)rows * slices * top * sizeof(uint64_t);
+}
+
+template <typename X>
+static void sc_launch_logprobs(const LogprobArgs& a, hipStream_t stream) {
+    const dim3 wg(SC_WG);
+    if (a.cols <= SC_WAVE_COLS) {
+        const dim3 grid(sc_grid((a.rows + SC_WAVES - 1) / SC_WAVES));
+        const int vecs = (a.cols + 64 * X::V - 1) / (64 * X::V);
+        if (vecs <= 1)
+            hipLaunchKernelGGL((k_token_logprobs_wave<X, 1>), grid, wg, 0, stream, a);
+        else if (vecs <= 2)
+            hipLaunchKernelGGL((k_token_logprobs_wave<X, 2>), grid, wg, 0, stream, a);
+        else if (vecs <= 4)
+            hipLaunchKernelGGL((k_token_logprobs_wave<X, 4>), grid, wg, 0, stream, a);
+        else
+            hipLaunchKernelGGL((k_token_logprobs_wave<X, SC_WAVE_COLS / 64 / X::V>), grid, wg, 0, stream, a);
+        return;
+    }
+    const dim3 grid(sc_grid(a.rows * a.slices));
+    if (a.top)
+        hipLaunchKernelGGL((k_token_logprobs_block<X, true>), grid, wg, 0, stream, a);
+    else
+        hipLaunchKernelGGL((k_token_logprobs_block<X, false>), grid, wg, 0, stream, a);
+    if (a.slices > 1) hipLaunchKernelGGL((k_token_logprobs_join<X>), dim3(sc_grid(a.rows)), wg, 0, stream, a);
+}
 
 extern "C" int pd_token_logprobs(const void* logits, int dtype, int64_t rows, int64_t columns, int64_t row_stride,
                                  const int32_t* widths, const int64_t* tokens, int n_tokens, int top, float* logp,
@@ -436,9 +1022,25 @@ extern "C" int pd_token_logprobs(const void* logits, int dtype, int64_t rows, in
     if (rc == 1) return PD_OK;
     if (n_tokens && (!tokens || !logp)) return sc_fail(fn, "tokens and logp are required with n_tokens");
     if (top && (!top_logp || !top_index)) return sc_fail(fn, "top_logp and top_index are required with top");
-    if (workspace_bytes < pd_token_logprobs_workspace(dtype, rows, columns, top)) return sc_fail(fn, "the workspace is too small");
+    const uint64_t need = pd_token_logprobs_workspace(dtype, rows, columns, top);
+    if (need && (!workspace || workspace_bytes < need)) {
+        pd_set_global_error("%s: a workspace of %llu bytes is needed", fn, (unsigned long long)need);
+        return PD_E_INVALID;
+    }
+    if (need && ((uintptr_t)workspace & 15)) return sc_fail(fn, "the workspace is not 16-byte aligned");
     LogprobArgs a = {logits, rows, row_stride, (int)columns, widths, tokens, n_tokens, top, logp, entropy, stats, top_logp, top_index};
-    SC_BY_TYPE(dtype, k_token_logprobs, sc_grid(rows), stream, a);
+    a.slices = 1;
+    if (columns > SC_WAVE_COLS) sc_slices(rows, columns, &a.slices, &a.slice_cols);
+    if (need) {
+        a.part = (Stat*)workspace;
+        a.part_keys = (uint64_t*)((char*)workspace + (((uint64_t)rows * a.slices * sizeof(Stat) + 15) & ~15ull));
+    }
+    if (dtype == PD_F32)
+        sc_launch_logprobs<F32>(a, (hipStream_t)stream);
+    else if (dtype == PD_BF16)
+        sc_launch_logprobs<BF16>(a, (hipStream_t)stream);
+    else
+        sc_launch_logprobs<F16>(a, (hipStream_t)stream);
     return sc_launched(fn);
 }
 
