@@ -678,112 +678,244 @@ struct LogprobGradArgs {
     int64_t out_stride;
 };
 
+// dx_j = -p_j (sum g + gH (log p_j + H)) + the tokens' own g, with t = log2 p_j = (x_j - m) log2 e - log2 S:
+// one read and one write of the row, some eleven instructions a score, bound by the memory.  A lane holds a token
+// (n_tok <= 64), so that the row's scores are compared with none: the one lane that holds a token's column adds
+// its g before the value is rounded, the tokens in their order.
+struct GradRow {
+    float base, log2_sum, c0, c1;  // dx = -p (c0 + c1 t)
+    bool empty;
+    int tok;      // this lane's token, -1: none, or not in the row
+    float g;
+};
+
+__device__ __forceinline__ GradRow sc_grad_row(const LogprobGradArgs& a, int64_t r, int n, int lane) {
+    GradRow q;
+    const float m = a.stats[3 * r], log_sum = a.stats[3 * r + 1], h = a.stats[3 * r + 2];
+    const float ge = a.g_entropy ? a.g_entropy[r] : 0.0f;
+    q.empty = m == -INFINITY && log_sum == 0;
+    q.base = m;
+    q.log2_sum = log_sum * SC_LOG2E;
+    q.tok = -1;
+    q.g = 0;
+    if (lane < a.n_tok) {
+        const int64_t tok = a.tokens[r * a.n_tok + lane];
+        if (tok >= 0) q.g = a.g_logp[r * a.n_tok + lane];
+        if (tok >= 0 && tok < n) q.tok = (int)tok;
+    }
+    q.c0 = fmaf(ge, h, a.n_tok > 1 ? sc_wave(q.g, SumOp()) : __shfl(q.g, 0));
+    q.c1 = ge * SC_LN2;
+    return q;
+}
+
+// The gradient of NV vectors of V columns, vector u at at0 + u * step, from the scores f, in their place.
+template <typename X, int NV>
+__device__ __forceinline__ void sc_grad_values(const LogprobGradArgs& a, const GradRow& q, int n, float* f, int at0, int step,
+                                               int begin, int end) {
+    constexpr int V = X::V;
+#pragma unroll
+    for (int i = 0; i < NV * V; ++i) {
+        const float t = fmaf(f[i] - q.base, SC_LOG2E, -q.log2_sum);
+        f[i] = -__builtin_amdgcn_exp2f(t) * fmaf(q.c1, sc_floor_t(t), q.c0);
+    }
+    for (int k = 0; k < a.n_tok; ++k) {
+        const int tok = __builtin_amdgcn_readlane(q.tok, k);
+        if (tok < begin || tok >= end) continue;
+        const float g = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(q.g), k));
+#pragma unroll
+        for (int i = 0; i < NV * V; ++i)
+            if (tok == at0 + (i / V) * step + i % V) f[i] += g;
+    }
+}
+
 template <typename X>
-__global__ __launch_bounds__(SC_WG) void k_token_logprobs_grad(LogprobGradArgs a) {
-    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+__device__ __forceinline__ void sc_grad_store(typename X::E* out, int at, int n, int cols, bool empty, float* f) {
+    constexpr int V = X::V;
+    if (empty || at + V > n)
+#pragma unroll
+        for (int e = 0; e < V; ++e) f[e] = empty || at + e >= n ? 0.0f : f[e];
+    if (at + V <= cols) {
+        sc_store<X>(out + at, X::pack(f));
+    } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+            if (at + e < cols) X::put(out + at + e, f[e]);
+    }
+}
+
+template <typename X, int NV>
+__global__ __launch_bounds__(SC_WG) void k_token_logprobs_grad_wave(LogprobGradArgs a) {
+    constexpr int V = X::V;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    for (int64_t r = (int64_t)blockIdx.x * SC_WAVES + wave; r < a.rows; r += (int64_t)gridDim.x * SC_WAVES) {
         const typename X::E* x = (const typename X::E*)a.x + r * a.stride;
         typename X::E* out = (typename X::E*)a.out + r * a.out_stride;
         const int n = sc_width(a.widths, r, a.cols);
-        const float m = a.stats[3 * r], log_sum = a.stats[3 * r + 1], h = a.stats[3 * r + 2];
-        const bool empty = m == -INFINITY && log_sum == 0;
-        const float ge = a.g_entropy ? a.g_entropy[r] : 0.0f;
-        float g = 0;
-        for (int t = 0; t < a.n_tok; ++t)
-            if (a.tokens[r * a.n_tok + t] >= 0) g += a.g_logp[r * a.n_tok + t];
-        for (int j = threadIdx.x; j < a.cols; j += SC_WG) {
-            float d = 0;
-            if (j < n && !empty) {
-                const float lp = (X::get(x + j) - m) - log_sum, p = exp2f(lp * SC_LOG2E);
-                d = -p * (g + ge * (fmaxf(lp, -256.0f) + h));
-                for (int t = 0; t < a.n_tok; ++t)
-                    if (a.tokens[r * a.n_tok + t] == j) d += a.g_logp[r * a.n_tok + t];
-            }
-            X::put(out + j, d);
+        float f[NV * V];
+#pragma unroll
+        for (int u = 0; u < NV; ++u) sc_read<X>(x, (u * 64 + lane) * V, n, f + u * V);
+        const GradRow q = sc_grad_row(a, r, n, lane);
+        sc_grad_values<X, NV>(a, q, n, f, lane * V, 64 * V, 0, a.cols);
+#pragma unroll
+        for (int u = 0; u < NV; ++u) sc_grad_store<X>(out, (u * 64 + lane) * V, n, a.cols, q.empty, f + u * V);
+    }
+}
+
+template <typename X>
+__global__ __launch_bounds__(SC_WG) void k_token_logprobs_grad_block(LogprobGradArgs a) {
+    constexpr int V = X::V, NV = SC_PER_THREAD / V;
+    const int t = threadIdx.x;
+    const int chunks = (a.cols + SC_CHUNK - 1) / SC_CHUNK;
+    for (int64_t b = blockIdx.x; b < a.rows * chunks; b += gridDim.x) {
+        const int64_t r = b / chunks;
+        const int at0 = (int)(b - r * chunks) * SC_CHUNK;
+        const typename X::E* x = (const typename X::E*)a.x + r * a.stride;
+        typename X::E* out = (typename X::E*)a.out + r * a.out_stride;
+        const int n = sc_width(a.widths, r, a.cols);
+        const bool whole = at0 + SC_CHUNK <= n;
+        float f[SC_PER_THREAD];
+        if (whole) {
+            sc_u4 w[NV];
+#pragma unroll
+            for (int u = 0; u < NV; ++u) w[u] = sc_load<X>(x + at0 + (u * SC_WG + t) * V);
+#pragma unroll
+            for (int u = 0; u < NV; ++u) X::unpack(w[u], f + u * V);
+        } else {
+#pragma unroll
+            for (int u = 0; u < NV; ++u) sc_read<X>(x, at0 + (u * SC_WG + t) * V, n, f + u * V);
+        }
+        const GradRow q = sc_grad_row(a, r, n, t & 63);
+        sc_grad_values<X, NV>(a, q, n, f, at0 + t * V, SC_WG * V, at0, at0 + SC_CHUNK);
+        if (whole && !q.empty) {
+#pragma unroll
+            for (int u = 0; u < NV; ++u) sc_store<X>(out + at0 + (u * SC_WG + t) * V, X::pack(f + u * V));
+        } else {
+#pragma unroll
+            for (int u = 0; u < NV; ++u) sc_grad_store<X>(out, at0 + (u * SC_WG + t) * V, n, a.cols, q.empty, f + u * V);
         }
     }
 }
 
 // ---- routing -------------------------------------------------------------------------------
 
+//
+// The order of the experts is that of float64 arithmetic, so that it does not depend on how a kernel forms its sums.
+// Without a bias it is the order of the logits, which float32 holds exactly.  With one, the scores p + bias are formed
+// in float32 with a known error; a row in which that error could decide is done again in float64 (k_route calls
+// sc_route_row for it, a wavefront to the row).  The same goes for the groups.
+//
+// A row belongs to L lanes (a power of two, whole groups to whole lanes), a lane holds EPL consecutive experts of one
+// group, a wavefront 64 / L rows.  A score and its place are one float64: the score's 24 bits fill the top of the
+// mantissa, the place goes to the bottom, so that one v_max_f64 orders both and no two are equal.  A lane sorts its
+// experts KP at a time by a bitonic network, keeps the best KP, and the lanes merge theirs in log2 L exchanges.  Bound
+// by instruction issue: some 70 instructions a row of 128 experts for its best eight.
+
 struct RouteArgs {
     const void* x;
+    int dtype;
     int64_t rows, stride;
     int experts, top, sigmoid;
     const float* bias;
-    int groups, top_groups, top2, renorm;
+    int groups, per_group, top_groups, top2, renorm;
     float scale;
     float* weights;
     int32_t* index;
+    int lanes, group_lanes;  // to a row, to a group
 };
 
-#define SC_PER_LANE (PD_MAX_EXPERTS / 64)
+__device__ __forceinline__ float sc_logit(const void* x, int dtype, int64_t at) {
+    if (dtype == PD_F32) return F32::get((const float*)x + at);
+    if (dtype == PD_BF16) return BF16::get((const uint16_t*)x + at);
+    return F16::get((const _Float16*)x + at);
+}
 
-// The weights of the chosen experts of one row; lane i < top holds the i-th one's logit.
-__device__ __forceinline__ void sc_route_weights(const RouteArgs& a, int64_t r, int lane, int idx, float xi, float m,
-                                                 float total) {
-    const bool have = lane < a.top;
-    float wgt;
-    if (a.sigmoid) {
-        float big = sc_wave(have ? xi : -INFINITY, MaxOp());
-        // a sum of tiny values is formed relative to the largest of them
-        const float shift = a.renorm && big < 0 && big > -INFINITY ? big : 0.0f;
-        wgt = xi < 0 ? expf(xi - shift) / (1 + expf(xi)) : 1 / (1 + expf(-xi));
-    } else if (a.renorm) {
-        float big = sc_wave(have ? xi : -INFINITY, MaxOp());
-        wgt = big == -INFINITY ? 0.0f : expf(xi - big);
+// Over the `lanes` lanes of a row, every lane of the wavefront taking part.
+template <typename T, typename F>
+__device__ __forceinline__ T sc_lanes(T v, int lanes, F f) {
+    if (lanes > 1) v = f(v, sc_across<1>(v));
+    if (lanes > 2) v = f(v, sc_across<2>(v));
+    if (lanes > 4) v = f(v, sc_across<4>(v));
+    if (lanes > 8) v = f(v, sc_across<8>(v));
+    if (lanes > 16) v = f(v, sc_across<16>(v));
+    if (lanes > 32) v = f(v, sc_across<32>(v));
+    return v;
+}
+
+// p of a chosen expert relative to the others': lane i < top of a row's lanes holds the i-th one's logit (-inf: none).
+// Sums of tiny sigmoids are formed relative to the largest, so that they do not all come to 0.
+__device__ __forceinline__ float sc_chosen_share(float xi, bool have, int sigmoid, int renorm, int lanes) {
+    float w;
+    if (sigmoid) {
+        float shift = 0;
+        if (renorm) {
+            const float big = sc_lanes(have ? xi : -INFINITY, lanes, FMaxOp());
+            if (big < 0 && big > -INFINITY) shift = big;
+        }
+        w = xi < 0 ? expf(xi - shift) / (1 + expf(xi)) : 1 / (1 + expf(-xi));
     } else {
-        wgt = total == 0 ? 0.0f : expf(xi - m) / total;
+        const float big = sc_lanes(have ? xi : -INFINITY, lanes, FMaxOp());
+        w = big == -INFINITY ? 0.0f : expf(xi - big);
     }
-    if (!have) wgt = 0;
-    if (a.renorm) {
-        const float sum = sc_wave(wgt, SumOp());
-        wgt = sum == 0 ? 0.0f : wgt / sum;
+    if (!have) w = 0;
+    if (renorm) {
+        const float sum = sc_lanes(w, lanes, SumOp());
+        w = sum == 0 ? 0.0f : w / sum;
     }
+    return w;
+}
+
+// Lane i < top of the `lanes` lanes of a row writes the i-th expert and its weight; m and total: the softmax's, where it
+// is not renormalised.
+__device__ __forceinline__ void sc_route_put(const RouteArgs& a, int64_t r, int i, int lanes, bool have, int idx, float m, float total) {
+    have &= i < a.top;
+    const float xi = have && idx >= 0 ? sc_logit(a.x, a.dtype, r * a.stride + idx) : -INFINITY;
+    float w;
+    if (a.sigmoid || a.renorm)
+        w = sc_chosen_share(xi, have, a.sigmoid, a.renorm, lanes);
+    else
+        w = total == 0 ? 0.0f : expf(xi - m) / total;
     if (have) {
-        a.weights[r * a.top + lane] = idx < 0 ? NAN : wgt * a.scale;
-        a.index[r * a.top + lane] = idx;
+        a.weights[r * a.top + i] = idx < 0 ? NAN : w * a.scale;
+        a.index[r * a.top + i] = idx;
     }
 }
 
-// One row by one wavefront, the order decided in float64.
-template <typename X>
-__device__ void sc_route_row(const RouteArgs& a, int64_t r, int lane) {
-    const typename X::E* x = (const typename X::E*)a.x + r * a.stride;
-    const int E = a.experts, per_group = E / a.groups;
-    float m = -INFINITY;
-    bool nan = false;
-    for (int j = lane; j < E; j += 64) {
-        const float v = X::get(x + j);
-        nan |= v != v || (v == INFINITY && !a.sigmoid);
-        m = fmaxf(m, v);
+// A row by one wavefront in float64.
+struct RouteExact {
+    const RouteArgs& a;
+    int64_t row;
+    double m, total;
+
+    __device__ double p(int j) const {
+        const double v = sc_logit(a.x, a.dtype, row + j);
+        if (a.sigmoid) return 1 / (1 + exp(-v));
+        return total > 0 ? exp(v - m) / total : 0.0;
     }
-    nan = __any(nan);
-    m = sc_wave(m, MaxOp());
-    double total = 0;
-    if (!a.sigmoid && m > -INFINITY)
-        for (int j = lane; j < E; j += 64) total += exp((double)X::get(x + j) - m);
-    total = sc_wave(total, SumOp());
-    double p[SC_PER_LANE], by[SC_PER_LANE];
-#pragma unroll
-    for (int i = 0; i < SC_PER_LANE; ++i) {
-        const int j = lane + 64 * i;
-        p[i] = by[i] = -INFINITY;
-        if (j >= E) continue;
-        const double v = X::get(x + j);
-        p[i] = a.sigmoid ? 1 / (1 + exp(-v)) : total > 0 ? exp(v - m) / total : 0.0;
-        by[i] = a.bias ? p[i] + (double)a.bias[j] : v;
-        if (!(by[i] >= -1e300)) by[i] = -1e300;  // -inf or NaN: behind every other, before what no group offers
+    // what the experts are ordered by; -inf and NaN behind all others
+    __device__ double by(int j) const {
+        const double v = a.bias ? p(j) + (double)a.bias[j] : (double)sc_logit(a.x, a.dtype, row + j);
+        return v >= -1e300 ? v : -1e300;
     }
+};
+
+__device__ __forceinline__ void sc_route_row(const RouteArgs& a, int64_t r, int lane) {
+    RouteExact q = {a, r * a.stride, -INFINITY, 0};
+    const int E = a.experts;
+    if (!a.sigmoid) {
+        float m = -INFINITY;
+        for (int j = lane; j < E; j += 64) m = fmaxf(m, sc_logit(a.x, a.dtype, q.row + j));
+        q.m = sc_wave(m, FMaxOp());
+        if (q.m > -INFINITY)
+            for (int j = lane; j < E; j += 64) q.total += exp(sc_logit(a.x, a.dtype, q.row + j) - q.m);
+        q.total = sc_wave(q.total, SumOp());
+    }
+    uint64_t kept = ~0ull;
     if (a.groups > 1) {
-        // lane g holds group g's score
-        double mine = -INFINITY;
+        double mine = -INFINITY;  // lane g: group g's
         for (int g = 0; g < a.groups; ++g) {
             double b1 = -INFINITY, b2 = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < SC_PER_LANE; ++i) {
-                const int j = lane + 64 * i;
-                if (j >= E || j / per_group != g) continue;
-                const double v = a.top2 && !a.bias ? p[i] : by[i];
+            for (int j = g * a.per_group + lane; j < (g + 1) * a.per_group; j += 64) {
+                const double v = a.top2 && !a.bias ? q.p(j) : q.by(j);
                 b2 = fmax(b2, fmin(b1, v));
                 b1 = fmax(b1, v);
             }
@@ -793,49 +925,272 @@ __device__ void sc_route_row(const RouteArgs& a, int64_t r, int lane) {
                 b2 = fmax(fmin(b1, o1), fmax(b2, o2));
                 b1 = fmax(b1, o1);
             }
-            const double s = a.top2 && per_group > 1 ? b1 + b2 : b1;
-            if (lane == g) mine = s;
+            if (lane == g) mine = a.top2 && a.per_group > 1 ? b1 + b2 : b1;
         }
         int rank = 0;
         for (int g = 0; g < a.groups; ++g) {
             const double o = __shfl(mine, g);
             rank += o > mine || (o == mine && g < lane);
         }
-        const uint64_t kept = __ballot(lane < a.groups && rank < a.top_groups);
-#pragma unroll
-        for (int i = 0; i < SC_PER_LANE; ++i) {
-            const int j = lane + 64 * i;
-            if (j < E && !(kept >> (j / per_group) & 1)) by[i] = -INFINITY;
-        }
+        kept = __ballot(lane < a.groups && rank < a.top_groups);
     }
-    int chosen = -1;
+    int chosen = -1, last_at = -1;
+    double last = INFINITY;
     for (int k = 0; k < a.top; ++k) {
         double best = -INFINITY;
         int at = E;
-#pragma unroll
-        for (int i = 0; i < SC_PER_LANE; ++i)
-            if (by[i] > best) best = by[i], at = lane + 64 * i;
+        for (int j = lane; j < E; j += 64) {
+            if (!(kept >> (j / a.per_group) & 1)) continue;
+            const double v = q.by(j);
+            if ((v < last || (v == last && j > last_at)) && v > best) best = v, at = j;
+        }
 #pragma unroll
         for (int d = 32; d; d >>= 1) {
             const double o = __shfl_xor(best, d);
             const int oa = __shfl_xor(at, d);
             if (o > best || (o == best && oa < at)) best = o, at = oa;
         }
-#pragma unroll
-        for (int i = 0; i < SC_PER_LANE; ++i)
-            if (lane + 64 * i == at) by[i] = -INFINITY;
+        last = best;
+        last_at = at;
         if (lane == k) chosen = at;
     }
-    const int idx = nan ? -1 : chosen;
-    const float xi = lane < a.top && idx >= 0 ? X::get(x + idx) : -INFINITY;
-    sc_route_weights(a, r, lane, idx, xi, m, (float)total);
+    sc_route_put(a, r, lane, 64, true, chosen, q.m == -INFINITY ? 0.0f : (float)q.m, (float)q.total);
 }
 
-template <typename X>
+// ---- sorting networks: descending, indexes known at compile time ------------------------------------
+
+__device__ __forceinline__ void sc_exchange(double& a, double& b) {  // the larger first
+    const double hi = fmax(a, b), lo = fmin(a, b);
+    a = hi;
+    b = lo;
+}
+// A bitonic sequence into descending order.
+template <int N>
+__device__ __forceinline__ void sc_bitonic(double* v) {
+    if constexpr (N > 1) {
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) sc_exchange(v[i], v[i + N / 2]);
+        sc_bitonic<N / 2>(v);
+        sc_bitonic<N / 2>(v + N / 2);
+    }
+}
+template <int N>
+__device__ __forceinline__ void sc_sort(double* v) {
+    if constexpr (N > 1) {
+        sc_sort<N / 2>(v);
+        sc_sort<N / 2>(v + N / 2);
+        // two descending halves: the first step compares ends with ends, what is left is bitonic
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) sc_exchange(v[i], v[N - 1 - i]);
+        sc_bitonic<N / 2>(v);
+        sc_bitonic<N / 2>(v + N / 2);
+    }
+}
+// The N largest of two descending lists, descending, into a.
+template <int N>
+__device__ __forceinline__ void sc_merge(double* a, const double* b) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) a[i] = fmax(a[i], b[N - 1 - i]);
+    sc_bitonic<N>(a);
+}
+template <int N, int STEP>
+__device__ __forceinline__ void sc_merge_across(double* a) {
+    double b[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) b[i] = sc_across<STEP>(a[i]);
+    sc_merge<N>(a, b);
+}
+
+// Score and place as one number.  Scores of +-inf go to +-2^1000, beyond every float32, a NaN to the lower one.
+__device__ __forceinline__ double sc_route_key(float s, int place) {
+    const double d = fmin(fmax((double)(s + 0.0f), -0x1p1000), 0x1p1000);
+    const uint64_t u = __double_as_longlong(d);
+    // of two equal negative numbers the one with the smaller magnitude is the larger
+    const uint32_t tail = (uint32_t)place ^ (~(uint32_t)((int64_t)u >> 63) & (PD_MAX_EXPERTS - 1));
+    return __longlong_as_double(u | tail);
+}
+__device__ __forceinline__ int sc_route_place(double key) {
+    const uint64_t u = __double_as_longlong(key);
+    return (int)(((uint32_t)u ^ ~(uint32_t)((int64_t)u >> 63)) & (PD_MAX_EXPERTS - 1));
+}
+
+// `have` consecutive logits from x + at on, -inf behind them.
+template <typename X, int EPL>
+__device__ __forceinline__ void sc_route_read(const void* base, int64_t at, int have, float* f) {
+    const typename X::E* x = (const typename X::E*)base + at;
+#pragma unroll
+    for (int u = 0; u < EPL / X::V; ++u) sc_read<X>(x, u * X::V, have, f + u * X::V);
+}
+
+template <int EPL, int KP, bool BIAS>
 __global__ __launch_bounds__(SC_WG) void k_route(RouteArgs a) {
-    const int lane = threadIdx.x & 63;
-    for (int64_t r = (int64_t)blockIdx.x * (SC_WG / 64) + (threadIdx.x >> 6); r < a.rows; r += (int64_t)gridDim.x * (SC_WG / 64))
-        sc_route_row<X>(a, r, lane);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int L = a.lanes, l = lane & (L - 1), first = lane & ~(L - 1), per_wave = 64 / L;
+    const int g = l / a.group_lanes, in_group = (l & (a.group_lanes - 1)) * EPL;
+    const int place = g * a.per_group + in_group;
+    const int room = g < a.groups ? pd_clampi(a.per_group - in_group, 0, EPL) : 0;
+    float bias[BIAS ? EPL : 1];
+    if constexpr (BIAS) {
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) bias[j] = j < room ? a.bias[place + j] : 0.0f;
+    }
+    const bool by_p = BIAS || (a.groups > 1 && a.top2);   // p takes part in the order
+    const bool want_p = by_p || !(a.sigmoid || a.renorm);  // p, or the softmax's sum, is needed
+    const int64_t tiles = (a.rows + per_wave - 1) / per_wave;
+    for (int64_t tile = (int64_t)blockIdx.x * SC_WAVES + wave; tile < tiles; tile += (int64_t)gridDim.x * SC_WAVES) {
+        const int64_t r = tile * per_wave + lane / L;
+        const bool on = r < a.rows;
+        const int have = on ? room : 0;
+        const int64_t at = on ? r * a.stride + place : 0;
+        float x[EPL], s[EPL];
+        if (a.dtype == PD_F32)
+            sc_route_read<F32, EPL>(a.x, at, have, x);
+        else if (a.dtype == PD_BF16)
+            sc_route_read<BF16, EPL>(a.x, at, have, x);
+        else
+            sc_route_read<F16, EPL>(a.x, at, have, x);
+        // rows without an order: NaN anywhere, +inf under a softmax
+        bool bad = false;
+        const int none = a.sigmoid ? 0x003 : 0x203;
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) bad |= __builtin_amdgcn_classf(x[j], none);
+        bad = (__ballot(bad) >> first & (L == 64 ? ~0ull : (1ull << L) - 1)) != 0;
+
+        float m = 0, total = 0, tol = 0;
+        if (want_p) {
+            if (a.sigmoid) {
+#pragma unroll
+                for (int j = 0; j < EPL; ++j) s[j] = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-SC_LOG2E * x[j]));
+                // error of p: p (1 - p) (|x| u ..) from the exponent, a step each for the exponential, the sum and
+                // the reciprocal, below 4 u; of a difference twice that (u = 2^-24)
+                tol = 0x1p-21f;
+            } else {
+                m = sc_lanes(sc_max<EPL>(x, -INFINITY), L, FMaxOp());
+                const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+                for (int j = 0; j < EPL; ++j) {
+                    s[j] = __builtin_amdgcn_exp2f((x[j] - base) * SC_LOG2E);
+                    total += s[j];
+                }
+                total = sc_lanes(total, L, SumOp());
+                const float inv = total == 0 ? 0.0f : 1.0f / total;
+#pragma unroll
+                for (int j = 0; j < EPL; ++j) s[j] *= inv;
+                // the largest p is 1 / total; every p is off by at most (EPL + 30) u of it: the sum's EPL + 6 steps,
+                // the exponents' |t| 2^t, the exponential, the division; of a difference twice that
+                tol = 0x1p-17f * inv;
+            }
+        }
+        if constexpr (BIAS) {
+#pragma unroll
+            for (int j = 0; j < EPL; ++j) s[j] += bias[j];
+        }
+        bool again = false, kept = true;
+        if (a.groups > 1) {
+            float b1 = -INFINITY, b2 = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < EPL; ++j) {
+                const float v = j < have ? (by_p ? s[j] : x[j]) : -INFINITY;
+                b2 = fmaxf(b2, fminf(b1, v));
+                b1 = fmaxf(b1, v);
+            }
+#define SC_TOP2_STEP(d)                                                 \
+    if (a.group_lanes > d) {                                            \
+        const float o1 = sc_across<d>(b1), o2 = sc_across<d>(b2);       \
+        b2 = fmaxf(fminf(b1, o1), fmaxf(b2, o2));                       \
+        b1 = fmaxf(b1, o1);                                             \
+    }
+            SC_TOP2_STEP(1) SC_TOP2_STEP(2) SC_TOP2_STEP(4) SC_TOP2_STEP(8) SC_TOP2_STEP(16) SC_TOP2_STEP(32)
+#undef SC_TOP2_STEP
+            const float mine = a.top2 && a.per_group > 1 ? b1 + b2 : b1;
+            if (by_p) {
+                const float off = 2 * tol + 0x1p-21f * fabsf(mine);
+                int above = 0, maybe = 0;
+                for (int k = 0; k < a.groups; ++k) {
+                    const float o = __shfl(mine, first + k * a.group_lanes);
+                    above += o > mine + off;
+                    maybe += k != g && !(o < mine - off);
+                }
+                kept = maybe < a.top_groups;
+                again = g < a.groups && !kept && above < a.top_groups;
+            } else {
+                int rank = 0;
+                for (int k = 0; k < a.groups; ++k) {
+                    const float o = __shfl(mine, first + k * a.group_lanes);
+                    rank += o > mine || (o == mine && k < g);
+                }
+                kept = rank < a.top_groups;
+            }
+        }
+        double best[KP];
+        {
+            constexpr int B = KP < EPL ? KP : EPL;
+#pragma unroll
+            for (int b = 0; b < EPL; b += B) {
+                double v[B];
+#pragma unroll
+                for (int j = 0; j < B; ++j)
+                    v[j] = kept && b + j < have ? sc_route_key(BIAS ? s[b + j] : x[b + j], place + b + j) : -INFINITY;
+                sc_sort<B>(v);
+                if (b == 0) {
+#pragma unroll
+                    for (int j = 0; j < KP; ++j) best[j] = j < B ? v[j < B ? j : 0] : -INFINITY;
+                } else if constexpr (B == KP) {
+                    sc_merge<KP>(best, v);
+                }
+            }
+        }
+        if (L > 1) sc_merge_across<KP, 1>(best);
+        if (L > 2) sc_merge_across<KP, 2>(best);
+        if (L > 4) sc_merge_across<KP, 4>(best);
+        if (L > 8) sc_merge_across<KP, 8>(best);
+        if (L > 16) sc_merge_across<KP, 16>(best);
+        if (L > 32) sc_merge_across<KP, 32>(best);
+
+        double mine = best[0], last = best[0];
+#pragma unroll
+        for (int k = 1; k < KP; ++k) {
+            mine = l == k ? best[k] : mine;
+            last = a.top - 1 == k ? best[k] : last;
+        }
+        if constexpr (BIAS) {
+            // Two neighbours in the list that are too close: in order if they are equal by logit and bias.
+            uint32_t close = 0;
+#pragma unroll
+            for (int k = 0; k + 1 < KP; ++k)
+                if (k + 1 < a.top && !(best[k] - best[k + 1] > tol + 0x1p-22 * fabs(best[k]))) close |= 1u << k;
+            if (on && !bad && close) {
+#pragma unroll
+                for (int k = 0; k + 1 < KP; ++k)
+                    if (close >> k & 1) {
+                        const int p0 = sc_route_place(best[k]), p1 = sc_route_place(best[k + 1]);
+                        again |= sc_logit(a.x, a.dtype, r * a.stride + p0) != sc_logit(a.x, a.dtype, r * a.stride + p1) ||
+                                 a.bias[p0] != a.bias[p1];
+                    }
+            }
+            // An expert too close to the last one chosen, on either side: the choice stands if they are equal.
+            const float edge = (float)last, off = tol + 0x1p-22f * fabsf(edge);
+            bool near = false;
+#pragma unroll
+            for (int j = 0; j < EPL; ++j) near |= j < have && kept && !(fabsf(s[j] - edge) > off);
+            if (on && !bad && near) {
+                const int pl = sc_route_place(last);
+                const float xl = sc_logit(a.x, a.dtype, r * a.stride + pl), bl = a.bias[pl];
+#pragma unroll
+                for (int j = 0; j < EPL; ++j)
+                    again |= j < have && !(fabsf(s[j] - edge) > off) && place + j != pl && (x[j] != xl || bias[j] != bl);
+            }
+        }
+        uint64_t todo = __ballot(again && on && !bad);
+        const uint64_t row_lanes = L == 64 ? ~0ull : (1ull << L) - 1;
+        const bool put = on && !(todo >> first & row_lanes);
+        sc_route_put(a, r, l, L, put, bad ? -1 : sc_route_place(mine), m == -INFINITY ? 0.0f : m, total);
+        while (todo) {  // rows whose order float32 does not tell: here, where the sorting's registers are free again
+            const int from = (__ffsll((unsigned long long)todo) - 1) & ~(L - 1);
+            sc_route_row(a, tile * per_wave + from / L, lane);
+            todo &= ~(row_lanes << from);
+        }
+    }
 }
 
 struct RouteGradArgs {
@@ -863,20 +1218,8 @@ __global__ __launch_bounds__(SC_WG) void k_route_grad(RouteGradArgs a) {
         const bool dense = !a.sigmoid && !a.renorm;
         float m = 0, total = 0, wgt, c;
         if (a.sigmoid || a.renorm) {
-            const float big = sc_wave(xi, MaxOp());
-            if (a.sigmoid) {
-                const float shift = a.renorm && big < 0 && big > -INFINITY ? big : 0.0f;
-                wgt = xi < 0 ? expf(xi - shift) / (1 + expf(xi)) : 1 / (1 + expf(-xi));
-            } else {
-                wgt = big == -INFINITY ? 0.0f : expf(xi - big);
-            }
-            if (!have) wgt = 0;
-            float sum = 0;
-            if (a.renorm) {
-                sum = sc_wave(wgt, SumOp());
-                wgt = sum == 0 ? 0.0f : wgt / sum;
-                sum = sc_wave(wgt * g, SumOp());
-            }
+            wgt = sc_chosen_share(xi, have, a.sigmoid, a.renorm, 64);
+            const float sum = a.renorm ? sc_wave(wgt * g, SumOp()) : 0.0f;
             c = wgt * (g - sum);
             if (a.sigmoid) c *= xi > 0 ? expf(-xi) / (1 + expf(-xi)) : 1 / (1 + expf(xi));  // 1 - p
         } else {
@@ -1044,6 +1387,26 @@ extern "C" int pd_token_logprobs(const void* logits, int dtype, int64_t rows, in
     return sc_launched(fn);
 }
 
+template <typename X>
+static void sc_launch_logprobs_grad(const LogprobGradArgs& a, hipStream_t stream) {
+    const dim3 wg(SC_WG);
+    if (a.cols <= SC_WAVE_COLS) {
+        const dim3 grid(sc_grid((a.rows + SC_WAVES - 1) / SC_WAVES));
+        const int vecs = (a.cols + 64 * X::V - 1) / (64 * X::V);
+        if (vecs <= 1)
+            hipLaunchKernelGGL((k_token_logprobs_grad_wave<X, 1>), grid, wg, 0, stream, a);
+        else if (vecs <= 2)
+            hipLaunchKernelGGL((k_token_logprobs_grad_wave<X, 2>), grid, wg, 0, stream, a);
+        else if (vecs <= 4)
+            hipLaunchKernelGGL((k_token_logprobs_grad_wave<X, 4>), grid, wg, 0, stream, a);
+        else
+            hipLaunchKernelGGL((k_token_logprobs_grad_wave<X, SC_WAVE_COLS / 64 / X::V>), grid, wg, 0, stream, a);
+        return;
+    }
+    const int64_t chunks = (a.cols + SC_CHUNK - 1) / SC_CHUNK;
+    hipLaunchKernelGGL((k_token_logprobs_grad_block<X>), dim3(sc_grid(a.rows * chunks)), wg, 0, stream, a);
+}
+
 extern "C" int pd_token_logprobs_grad(const void* logits, int dtype, int64_t rows, int64_t columns, int64_t row_stride,
                                       const int32_t* widths, const float* stats, const int64_t* tokens, int n_tokens,
                                       const float* grad_logp, const float* grad_entropy, void* grad, int64_t grad_stride,
@@ -1057,7 +1420,12 @@ extern "C" int pd_token_logprobs_grad(const void* logits, int dtype, int64_t row
     if (n_tokens && (!tokens || !grad_logp)) return sc_fail(fn, "tokens and grad_logp are required with n_tokens");
     if (sc_check_grad(fn, logits, dtype, rows, columns, row_stride, grad, grad_stride)) return PD_E_INVALID;
     LogprobGradArgs a = {logits, rows, row_stride, (int)columns, widths, stats, tokens, n_tokens, grad_logp, grad_entropy, grad, grad_stride};
-    SC_BY_TYPE(dtype, k_token_logprobs_grad, sc_grid(rows), stream, a);
+    if (dtype == PD_F32)
+        sc_launch_logprobs_grad<F32>(a, (hipStream_t)stream);
+    else if (dtype == PD_BF16)
+        sc_launch_logprobs_grad<BF16>(a, (hipStream_t)stream);
+    else
+        sc_launch_logprobs_grad<F16>(a, (hipStream_t)stream);
     return sc_launched(fn);
 }
 
@@ -1065,6 +1433,39 @@ static int sc_check_route(const char* fn, int64_t experts, int top, int score) {
     if (score != PD_SCORE_SOFTMAX && score != PD_SCORE_SIGMOID) return sc_fail(fn, "score is PD_SCORE_SOFTMAX or PD_SCORE_SIGMOID");
     if (top < 1 || top > PD_MAX_ROUTES || top > experts) return sc_fail(fn, "top is outside 1..32 or larger than the number of experts");
     return 0;
+}
+
+static int sc_pow2(int v) {
+    int p = 1;
+    while (p < v) p *= 2;
+    return p;
+}
+
+template <int EPL, bool BIAS>
+static void sc_launch_route_epl(const RouteArgs& a, int kp, unsigned grid, hipStream_t stream) {
+    const dim3 wg(SC_WG);
+    if (kp == 2)
+        hipLaunchKernelGGL((k_route<EPL, 2, BIAS>), dim3(grid), wg, 0, stream, a);
+    else if (kp == 4)
+        hipLaunchKernelGGL((k_route<EPL, 4, BIAS>), dim3(grid), wg, 0, stream, a);
+    else if (kp == 8)
+        hipLaunchKernelGGL((k_route<EPL, 8, BIAS>), dim3(grid), wg, 0, stream, a);
+    else if (kp == 16)
+        hipLaunchKernelGGL((k_route<EPL, 16, BIAS>), dim3(grid), wg, 0, stream, a);
+    else
+        hipLaunchKernelGGL((k_route<EPL, 32, BIAS>), dim3(grid), wg, 0, stream, a);
+}
+
+template <bool BIAS>
+static void sc_launch_route(const RouteArgs& a, int epl, int kp, hipStream_t stream) {
+    const int64_t rows_wg = 64 / a.lanes * SC_WAVES;
+    const unsigned grid = sc_grid((a.rows + rows_wg - 1) / rows_wg);
+    if (epl <= 8)
+        sc_launch_route_epl<8, BIAS>(a, kp, grid, stream);
+    else if (epl <= 16)
+        sc_launch_route_epl<16, BIAS>(a, kp, grid, stream);
+    else
+        sc_launch_route_epl<32, BIAS>(a, kp, grid, stream);
 }
 
 extern "C" int pd_route_experts(const void* logits, int dtype, int64_t rows, int64_t experts, int64_t row_stride,
@@ -1080,9 +1481,19 @@ extern "C" int pd_route_experts(const void* logits, int dtype, int64_t rows, int
     if (group_score != PD_GROUP_MAX && group_score != PD_GROUP_TOP2) return sc_fail(fn, "group_score is PD_GROUP_MAX or PD_GROUP_TOP2");
     if (rc == 1) return PD_OK;
     if (!weights || !index) return sc_fail(fn, "weights and index are required");
-    RouteArgs a = {logits, rows, row_stride, (int)experts, top, score == PD_SCORE_SIGMOID, bias, groups, top_groups,
-                   group_score == PD_GROUP_TOP2, renormalise != 0, scale, weights, index};
-    SC_BY_TYPE(dtype, k_route, sc_grid((rows + 3) / 4), stream, a);
+    RouteArgs a = {logits, dtype, rows, row_stride, (int)experts, top, score == PD_SCORE_SIGMOID, bias, groups, (int)experts / groups,
+                   top_groups, group_score == PD_GROUP_TOP2, renormalise != 0, scale, weights, index};
+    // The fewest lanes that hold a row (at most 32 experts each), a group each at least, and write its `top` results:
+    // a lane's work grows more slowly with its experts than the number of rows in a wavefront falls with its lanes.
+    const int kp = sc_pow2(top < 2 ? 2 : top), gp = sc_pow2(groups);
+    a.lanes = kp > gp ? kp : gp;
+    while (a.lanes / gp * 32 < a.per_group) a.lanes *= 2;
+    a.group_lanes = a.lanes / gp;
+    const int epl = (a.per_group + a.group_lanes - 1) / a.group_lanes;
+    if (bias)
+        sc_launch_route<true>(a, epl, kp, (hipStream_t)stream);
+    else
+        sc_launch_route<false>(a, epl, kp, (hipStream_t)stream);
     return sc_launched(fn);
 }
 
