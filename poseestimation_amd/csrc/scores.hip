@@ -121,37 +121,69 @@ __device__ __forceinline__ uint32_t sc_dpp(uint32_t v) {
     return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
 }
 
-// v of the lane STEP away in a butterfly; once the lanes of a group of STEP hold the same value any lane of the
-// neighbouring group will do, which is what lets the row mirrors stand in for the exchanges at 4 and 8.
+// One step of a butterfly: p and q are v of the two neighbouring groups of STEP lanes, in the same order for both.
+// Within a group of STEP lanes v is the same already, so that any lane of the other group will do: the row mirrors stand
+// in for the exchanges at 4 and 8, and the row swaps of v with itself give both sides at 16 and 32.  (An exchange through
+// LDS, as __shfl_xor, issues at a third of their rate.)
 template <int STEP>
-__device__ __forceinline__ uint32_t sc_across(uint32_t v) {
-    if (STEP == 1) return sc_dpp<0xB1>(v);   // quad_perm 1 0 3 2
-    if (STEP == 2) return sc_dpp<0x4E>(v);   // quad_perm 2 3 0 1
-    if (STEP == 4) return sc_dpp<0x141>(v);  // row_half_mirror
-    if (STEP == 8) return sc_dpp<0x140>(v);  // row_mirror
-    return (uint32_t)__shfl_xor((int)v, STEP);
+__device__ __forceinline__ void sc_pair(uint32_t v, uint32_t& p, uint32_t& q) {
+    if constexpr (STEP >= 16) {
+        const auto both = STEP == 16 ? __builtin_amdgcn_permlane16_swap(v, v, false, false)
+                                     : __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        p = both[0];
+        q = both[1];
+    } else {
+        p = v;
+        q = STEP == 1 ? sc_dpp<0xB1>(v)     // quad_perm 1 0 3 2
+            : STEP == 2 ? sc_dpp<0x4E>(v)   // quad_perm 2 3 0 1
+            : STEP == 4 ? sc_dpp<0x141>(v)  // row_half_mirror
+                        : sc_dpp<0x140>(v); // row_mirror
+    }
 }
 template <int STEP>
-__device__ __forceinline__ float sc_across(float v) { return __uint_as_float(sc_across<STEP>(__float_as_uint(v))); }
-template <int STEP>
-__device__ __forceinline__ double sc_across(double v) {
-    const uint64_t u = __double_as_longlong(v);
-    return __longlong_as_double((uint64_t)sc_across<STEP>((uint32_t)(u >> 32)) << 32 | sc_across<STEP>((uint32_t)u));
+__device__ __forceinline__ void sc_pair(float v, float& p, float& q) {
+    uint32_t a, b;
+    sc_pair<STEP>(__float_as_uint(v), a, b);
+    p = __uint_as_float(a);
+    q = __uint_as_float(b);
 }
 template <int STEP>
-__device__ __forceinline__ uint64_t sc_across(uint64_t u) {
-    return (uint64_t)sc_across<STEP>((uint32_t)(u >> 32)) << 32 | sc_across<STEP>((uint32_t)u);
+__device__ __forceinline__ void sc_pair(uint64_t v, uint64_t& p, uint64_t& q) {
+    uint32_t a, b, c, d;
+    sc_pair<STEP>((uint32_t)v, a, b);
+    sc_pair<STEP>((uint32_t)(v >> 32), c, d);
+    p = (uint64_t)c << 32 | a;
+    q = (uint64_t)d << 32 | b;
+}
+template <int STEP>
+__device__ __forceinline__ void sc_pair(double v, double& p, double& q) {
+    uint64_t a, b;
+    sc_pair<STEP>((uint64_t)__double_as_longlong(v), a, b);
+    p = __longlong_as_double(a);
+    q = __longlong_as_double(b);
+}
+template <int STEP, typename T, typename F>
+__device__ __forceinline__ T sc_step(T v, F f) {
+    T p, q;
+    sc_pair<STEP>(v, p, q);
+    return f(p, q);
 }
 
-// Over a whole wavefront, every lane taking part; all get the result.
+// Over the first `lanes` (a power of two) lanes and each further group of as many, every lane of the wavefront taking
+// part; all of a group get its result.
+template <typename T, typename F>
+__device__ __forceinline__ T sc_lanes(T v, int lanes, F f) {
+    if (lanes > 1) v = sc_step<1>(v, f);
+    if (lanes > 2) v = sc_step<2>(v, f);
+    if (lanes > 4) v = sc_step<4>(v, f);
+    if (lanes > 8) v = sc_step<8>(v, f);
+    if (lanes > 16) v = sc_step<16>(v, f);
+    if (lanes > 32) v = sc_step<32>(v, f);
+    return v;
+}
 template <typename T, typename F>
 __device__ __forceinline__ T sc_wave(T v, F f) {
-    v = f(v, sc_across<1>(v));
-    v = f(v, sc_across<2>(v));
-    v = f(v, sc_across<4>(v));
-    v = f(v, sc_across<8>(v));
-    v = f(v, sc_across<16>(v));
-    return f(v, sc_across<32>(v));
+    return sc_lanes(v, 64, f);
 }
 
 template <typename T, typename F>
@@ -805,10 +837,10 @@ __global__ __launch_bounds__(SC_WG) void k_token_logprobs_grad_block(LogprobGrad
 // sc_route_row for it, a wavefront to the row).  The same goes for the groups.
 //
 // A row belongs to L lanes (a power of two, whole groups to whole lanes), a lane holds EPL consecutive experts of one
-// group, a wavefront 64 / L rows.  A score and its place are one float64: the score's 24 bits fill the top of the
-// mantissa, the place goes to the bottom, so that one v_max_f64 orders both and no two are equal.  A lane sorts its
-// experts KP at a time by a bitonic network, keeps the best KP, and the lanes merge theirs in log2 L exchanges.  Bound
-// by instruction issue: some 70 instructions a row of 128 experts for its best eight.
+// group, a wavefront 64 / L rows.  A score and its place are one floating-point number, the place in mantissa bits that
+// the score does not use, so that one v_max orders both and no two are equal: bfloat16 and float16 logits leave 13 bits
+// of a float32, all else goes into a float64 (its v_max issues at the same rate).  A lane sorts its experts KP at a time by
+// a bitonic network, keeps the best KP, and the lanes merge theirs in log2 L exchanges.  Bound by instruction issue.
 
 struct RouteArgs {
     const void* x;
@@ -827,18 +859,6 @@ __device__ __forceinline__ float sc_logit(const void* x, int dtype, int64_t at) 
     if (dtype == PD_F32) return F32::get((const float*)x + at);
     if (dtype == PD_BF16) return BF16::get((const uint16_t*)x + at);
     return F16::get((const _Float16*)x + at);
-}
-
-// Over the `lanes` lanes of a row, every lane of the wavefront taking part.
-template <typename T, typename F>
-__device__ __forceinline__ T sc_lanes(T v, int lanes, F f) {
-    if (lanes > 1) v = f(v, sc_across<1>(v));
-    if (lanes > 2) v = f(v, sc_across<2>(v));
-    if (lanes > 4) v = f(v, sc_across<4>(v));
-    if (lanes > 8) v = f(v, sc_across<8>(v));
-    if (lanes > 16) v = f(v, sc_across<16>(v));
-    if (lanes > 32) v = f(v, sc_across<32>(v));
-    return v;
 }
 
 // p of a chosen expert relative to the others': lane i < top of a row's lanes holds the i-th one's logit (-inf: none).
@@ -864,14 +884,14 @@ __device__ __forceinline__ float sc_chosen_share(float xi, bool have, int sigmoi
     return w;
 }
 
-// Lane i < top of the `lanes` lanes of a row writes the i-th expert and its weight; m and total: the softmax's, where it
-// is not renormalised.
-__device__ __forceinline__ void sc_route_put(const RouteArgs& a, int64_t r, int i, int lanes, bool have, int idx, float m, float total) {
+// Lane i < top of the `lanes` lanes of a row writes the i-th expert and its weight, from its logit; m and total: the
+// softmax's, where it is not renormalised.  idx < 0: the row has no order.
+__device__ __forceinline__ void sc_route_put(const RouteArgs& a, int64_t r, int i, int lanes, bool have, int idx, float xi,
+                                             float m, float total) {
     have &= i < a.top;
-    const float xi = have && idx >= 0 ? sc_logit(a.x, a.dtype, r * a.stride + idx) : -INFINITY;
     float w;
     if (a.sigmoid || a.renorm)
-        w = sc_chosen_share(xi, have, a.sigmoid, a.renorm, lanes);
+        w = sc_chosen_share(have ? xi : -INFINITY, have, a.sigmoid, a.renorm, lanes);
     else
         w = total == 0 ? 0.0f : expf(xi - m) / total;
     if (have) {
@@ -880,52 +900,40 @@ __device__ __forceinline__ void sc_route_put(const RouteArgs& a, int64_t r, int 
     }
 }
 
-// A row by one wavefront in float64.
-struct RouteExact {
-    const RouteArgs& a;
-    int64_t row;
-    double m, total;
-
-    __device__ double p(int j) const {
-        const double v = sc_logit(a.x, a.dtype, row + j);
-        if (a.sigmoid) return 1 / (1 + exp(-v));
-        return total > 0 ? exp(v - m) / total : 0.0;
-    }
-    // what the experts are ordered by; -inf and NaN behind all others
-    __device__ double by(int j) const {
-        const double v = a.bias ? p(j) + (double)a.bias[j] : (double)sc_logit(a.x, a.dtype, row + j);
-        return v >= -1e300 ? v : -1e300;
-    }
-};
-
-__device__ __forceinline__ void sc_route_row(const RouteArgs& a, int64_t r, int lane) {
-    RouteExact q = {a, r * a.stride, -INFINITY, 0};
+// A row by one wavefront in float64; by: PD_MAX_EXPERTS values of the wavefront's own.
+__device__ __forceinline__ void sc_route_row(const RouteArgs& a, int64_t r, int lane, double* by) {
     const int E = a.experts;
+    const int64_t row = r * a.stride;
+    double m = 0, total = 0;
     if (!a.sigmoid) {
-        float m = -INFINITY;
-        for (int j = lane; j < E; j += 64) m = fmaxf(m, sc_logit(a.x, a.dtype, q.row + j));
-        q.m = sc_wave(m, FMaxOp());
-        if (q.m > -INFINITY)
-            for (int j = lane; j < E; j += 64) q.total += exp(sc_logit(a.x, a.dtype, q.row + j) - q.m);
-        q.total = sc_wave(q.total, SumOp());
+        float big = -INFINITY;
+        for (int j = lane; j < E; j += 64) big = fmaxf(big, sc_logit(a.x, a.dtype, row + j));
+        big = sc_wave(big, FMaxOp());
+        if (big > -INFINITY) {
+            m = big;
+            for (int j = lane; j < E; j += 64) total += exp(sc_logit(a.x, a.dtype, row + j) - m);
+        }
+        total = sc_wave(total, SumOp());
     }
+    const bool by_p = a.bias || (a.groups > 1 && a.top2);  // else by the logits alone
+    for (int j = lane; j < E; j += 64) {
+        const double x = sc_logit(a.x, a.dtype, row + j);
+        double v = x;
+        if (by_p) v = a.sigmoid ? 1 / (1 + exp(-x)) : total > 0 ? exp(x - m) / total : 0.0;
+        if (a.bias) v += a.bias[j];
+        by[j] = v >= -1e300 ? v : -1e300;  // -inf and NaN behind all others
+    }
+    pd_wave_sync();
     uint64_t kept = ~0ull;
     if (a.groups > 1) {
         double mine = -INFINITY;  // lane g: group g's
-        for (int g = 0; g < a.groups; ++g) {
+        if (lane < a.groups) {
             double b1 = -INFINITY, b2 = -INFINITY;
-            for (int j = g * a.per_group + lane; j < (g + 1) * a.per_group; j += 64) {
-                const double v = a.top2 && !a.bias ? q.p(j) : q.by(j);
-                b2 = fmax(b2, fmin(b1, v));
-                b1 = fmax(b1, v);
+            for (int j = lane * a.per_group; j < (lane + 1) * a.per_group; ++j) {
+                b2 = fmax(b2, fmin(b1, by[j]));
+                b1 = fmax(b1, by[j]);
             }
-#pragma unroll
-            for (int d = 32; d; d >>= 1) {
-                const double o1 = __shfl_xor(b1, d), o2 = __shfl_xor(b2, d);
-                b2 = fmax(fmin(b1, o1), fmax(b2, o2));
-                b1 = fmax(b1, o1);
-            }
-            if (lane == g) mine = a.top2 && a.per_group > 1 ? b1 + b2 : b1;
+            mine = a.top2 && a.per_group > 1 ? b1 + b2 : b1;
         }
         int rank = 0;
         for (int g = 0; g < a.groups; ++g) {
@@ -934,39 +942,42 @@ __device__ __forceinline__ void sc_route_row(const RouteArgs& a, int64_t r, int 
         }
         kept = __ballot(lane < a.groups && rank < a.top_groups);
     }
-    int chosen = -1, last_at = -1;
-    double last = INFINITY;
+    for (int j = lane; j < E; j += 64) {
+        if (by_p && !a.bias) by[j] = fmax((double)sc_logit(a.x, a.dtype, row + j), -1e300);  // p counted for the groups only
+        if (!(kept >> (j / a.per_group) & 1)) by[j] = -INFINITY;
+    }
+    int chosen = -1;
     for (int k = 0; k < a.top; ++k) {
         double best = -INFINITY;
         int at = E;
-        for (int j = lane; j < E; j += 64) {
-            if (!(kept >> (j / a.per_group) & 1)) continue;
-            const double v = q.by(j);
-            if ((v < last || (v == last && j > last_at)) && v > best) best = v, at = j;
-        }
-#pragma unroll
-        for (int d = 32; d; d >>= 1) {
-            const double o = __shfl_xor(best, d);
-            const int oa = __shfl_xor(at, d);
-            if (o > best || (o == best && oa < at)) best = o, at = oa;
-        }
-        last = best;
-        last_at = at;
+        for (int j = lane; j < E; j += 64)
+            if (by[j] > best) best = by[j], at = j;
+        const double top = sc_wave(best, MaxOp());
+        at = (int)sc_wave((uint32_t)(best == top ? at : E), MinOp());
+        if ((at & 63) == lane && at < E) by[at] = -INFINITY;
         if (lane == k) chosen = at;
     }
-    sc_route_put(a, r, lane, 64, true, chosen, q.m == -INFINITY ? 0.0f : (float)q.m, (float)q.total);
+    const float xi = lane < a.top ? sc_logit(a.x, a.dtype, row + chosen) : -INFINITY;
+    sc_route_put(a, r, lane, 64, true, chosen, xi, (float)m, (float)total);
+    pd_wave_sync();
 }
 
 // ---- sorting networks: descending, indexes known at compile time ------------------------------------
 
-__device__ __forceinline__ void sc_exchange(double& a, double& b) {  // the larger first
-    const double hi = fmax(a, b), lo = fmin(a, b);
+__device__ __forceinline__ double sc_hi(double a, double b) { return fmax(a, b); }
+__device__ __forceinline__ double sc_lo(double a, double b) { return fmin(a, b); }
+__device__ __forceinline__ float sc_hi(float a, float b) { return fmaxf(a, b); }
+__device__ __forceinline__ float sc_lo(float a, float b) { return fminf(a, b); }
+
+template <typename K>
+__device__ __forceinline__ void sc_exchange(K& a, K& b) {  // the larger first
+    const K hi = sc_hi(a, b), lo = sc_lo(a, b);
     a = hi;
     b = lo;
 }
 // A bitonic sequence into descending order.
-template <int N>
-__device__ __forceinline__ void sc_bitonic(double* v) {
+template <int N, typename K>
+__device__ __forceinline__ void sc_bitonic(K* v) {
     if constexpr (N > 1) {
 #pragma unroll
         for (int i = 0; i < N / 2; ++i) sc_exchange(v[i], v[i + N / 2]);
@@ -974,8 +985,8 @@ __device__ __forceinline__ void sc_bitonic(double* v) {
         sc_bitonic<N / 2>(v + N / 2);
     }
 }
-template <int N>
-__device__ __forceinline__ void sc_sort(double* v) {
+template <int N, typename K>
+__device__ __forceinline__ void sc_sort(K* v) {
     if constexpr (N > 1) {
         sc_sort<N / 2>(v);
         sc_sort<N / 2>(v + N / 2);
@@ -987,123 +998,165 @@ __device__ __forceinline__ void sc_sort(double* v) {
     }
 }
 // The N largest of two descending lists, descending, into a.
-template <int N>
-__device__ __forceinline__ void sc_merge(double* a, const double* b) {
+template <int N, typename K>
+__device__ __forceinline__ void sc_merge(K* a, const K* b) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) a[i] = fmax(a[i], b[N - 1 - i]);
+    for (int i = 0; i < N; ++i) a[i] = sc_hi(a[i], b[N - 1 - i]);
     sc_bitonic<N>(a);
 }
-template <int N, int STEP>
-__device__ __forceinline__ void sc_merge_across(double* a) {
-    double b[N];
+template <int N, int STEP, typename K>
+__device__ __forceinline__ void sc_merge_across(K* a) {
+    K p[N], q[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) b[i] = sc_across<STEP>(a[i]);
-    sc_merge<N>(a, b);
+    for (int i = 0; i < N; ++i) sc_pair<STEP>(a[i], p[i], q[i]);
+#pragma unroll
+    for (int i = 0; i < N; ++i) a[i] = p[i];
+    sc_merge<N>(a, q);
 }
 
-// Score and place as one number.  Scores of +-inf go to +-2^1000, beyond every float32, a NaN to the lower one.
-__device__ __forceinline__ double sc_route_key(float s, int place) {
-    const double d = fmin(fmax((double)(s + 0.0f), -0x1p1000), 0x1p1000);
-    const uint64_t u = __double_as_longlong(d);
-    // of two equal negative numbers the one with the smaller magnitude is the larger
-    const uint32_t tail = (uint32_t)place ^ (~(uint32_t)((int64_t)u >> 63) & (PD_MAX_EXPERTS - 1));
-    return __longlong_as_double(u | tail);
-}
-__device__ __forceinline__ int sc_route_place(double key) {
-    const uint64_t u = __double_as_longlong(key);
-    return (int)(((uint32_t)u ^ ~(uint32_t)((int64_t)u >> 63)) & (PD_MAX_EXPERTS - 1));
-}
+// Score and place as one number.  Of two equal scores the one of the lower place is the larger: where the number is
+// negative the one with the smaller magnitude.  -inf (float64: and NaN) comes behind every finite score.
+#define SC_PLACES (PD_MAX_EXPERTS - 1)
+struct Key32 {  // of a bfloat16 or float16 value: its float32 has 13 bits to spare, and no finite one reaches SC_INF32
+    typedef float K;
+    static constexpr uint32_t SC_INF32 = 0x7f7ffc00u;
+    static __device__ __forceinline__ K make(float s, int place) {
+        const float f = __builtin_amdgcn_fmed3f(s + 0.0f, -__uint_as_float(SC_INF32), __uint_as_float(SC_INF32));
+        const uint32_t u = __float_as_uint(f);
+        return __uint_as_float(u | ((uint32_t)place ^ (~(uint32_t)((int32_t)u >> 31) & SC_PLACES)));
+    }
+    static __device__ __forceinline__ int place(K key) {
+        const uint32_t u = __float_as_uint(key);
+        return (int)((u ^ ~(uint32_t)((int32_t)u >> 31)) & SC_PLACES);
+    }
+    static __device__ __forceinline__ float score(K key) {
+        const uint32_t u = __float_as_uint(key) & ~(uint32_t)SC_PLACES, mag = u & 0x7fffffffu;
+        return __uint_as_float(mag >= SC_INF32 ? (u & 0x80000000u) | 0x7f800000u : u);
+    }
+};
+struct Key64 {
+    typedef double K;
+    static __device__ __forceinline__ K make(float s, int place) {
+        const double d = fmin(fmax((double)(s + 0.0f), -0x1p1000), 0x1p1000);
+        const uint64_t u = __double_as_longlong(d);
+        return __longlong_as_double(u | ((uint32_t)place ^ (~(uint32_t)((int64_t)u >> 63) & SC_PLACES)));
+    }
+    static __device__ __forceinline__ int place(K key) {
+        const uint64_t u = __double_as_longlong(key);
+        return (int)(((uint32_t)u ^ ~(uint32_t)((int64_t)u >> 63)) & SC_PLACES);
+    }
+    static __device__ __forceinline__ float score(K key) {  // +-2^1000 rounds to +-inf
+        return (float)__longlong_as_double(__double_as_longlong(key) & ~(uint64_t)SC_PLACES);
+    }
+};
 
-// `have` consecutive logits from x + at on, -inf behind them.
+// `have` consecutive logits from element `at` on, -inf behind them.
 template <typename X, int EPL>
-__device__ __forceinline__ void sc_route_read(const void* base, int64_t at, int have, float* f) {
+__device__ __forceinline__ void sc_route_read(const void* base, int64_t at, int have, bool full, float* f) {
     const typename X::E* x = (const typename X::E*)base + at;
+    if (full) {
+        sc_u4 w[EPL / X::V];
 #pragma unroll
-    for (int u = 0; u < EPL / X::V; ++u) sc_read<X>(x, u * X::V, have, f + u * X::V);
+        for (int u = 0; u < EPL / X::V; ++u) w[u] = sc_load<X>(x + u * X::V);
+#pragma unroll
+        for (int u = 0; u < EPL / X::V; ++u) X::unpack(w[u], f + u * X::V);
+    } else {
+#pragma unroll
+        for (int u = 0; u < EPL / X::V; ++u) sc_read<X>(x, u * X::V, have, f + u * X::V);
+    }
 }
 
-template <int EPL, int KP, bool BIAS>
+// PLAIN16, PLAIN32: the order is that of the logits (no bias, no sums of two p for the groups), 16-bit or float32 ones.
+// CLOSE: p + bias, or groups by sums of p, take part in it, and close calls are taken to float64.
+enum { ROUTE_PLAIN16, ROUTE_PLAIN32, ROUTE_CLOSE };
+
+template <int EPL, int KP, int MODE>
 __global__ __launch_bounds__(SC_WG) void k_route(RouteArgs a) {
+    typedef typename std::conditional<MODE == ROUTE_PLAIN16, Key32, Key64>::type Key;
+    typedef typename Key::K K;
+    constexpr bool CLOSE = MODE == ROUTE_CLOSE;
+    __shared__ double by[CLOSE ? SC_WAVES : 1][CLOSE ? PD_MAX_EXPERTS : 1];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int L = a.lanes, l = lane & (L - 1), first = lane & ~(L - 1), per_wave = 64 / L;
+    const uint64_t row_lanes = (L == 64 ? ~0ull : (1ull << L) - 1) << first;
     const int g = l / a.group_lanes, in_group = (l & (a.group_lanes - 1)) * EPL;
     const int place = g * a.per_group + in_group;
-    const int room = g < a.groups ? pd_clampi(a.per_group - in_group, 0, EPL) : 0;
-    float bias[BIAS ? EPL : 1];
-    if constexpr (BIAS) {
+    const int have = g < a.groups ? pd_clampi(a.per_group - in_group, 0, EPL) : 0;
+    const bool full = __ballot(have == EPL) == ~0ull;
+    const bool biased = CLOSE && a.bias;
+    float bias[CLOSE ? EPL : 1];
+    if constexpr (CLOSE) {
 #pragma unroll
-        for (int j = 0; j < EPL; ++j) bias[j] = j < room ? a.bias[place + j] : 0.0f;
+        for (int j = 0; j < EPL; ++j) bias[j] = biased && j < have ? a.bias[place + j] : 0.0f;
     }
-    const bool by_p = BIAS || (a.groups > 1 && a.top2);   // p takes part in the order
-    const bool want_p = by_p || !(a.sigmoid || a.renorm);  // p, or the softmax's sum, is needed
     const int64_t tiles = (a.rows + per_wave - 1) / per_wave;
     for (int64_t tile = (int64_t)blockIdx.x * SC_WAVES + wave; tile < tiles; tile += (int64_t)gridDim.x * SC_WAVES) {
-        const int64_t r = tile * per_wave + lane / L;
+        const int64_t r = tile * per_wave + lane / L, row = r < a.rows ? r : a.rows - 1;
         const bool on = r < a.rows;
-        const int have = on ? room : 0;
-        const int64_t at = on ? r * a.stride + place : 0;
         float x[EPL], s[EPL];
-        if (a.dtype == PD_F32)
-            sc_route_read<F32, EPL>(a.x, at, have, x);
+        if (MODE == ROUTE_PLAIN32 || (CLOSE && a.dtype == PD_F32))
+            sc_route_read<F32, EPL>(a.x, row * a.stride + place, have, full, x);
         else if (a.dtype == PD_BF16)
-            sc_route_read<BF16, EPL>(a.x, at, have, x);
+            sc_route_read<BF16, EPL>(a.x, row * a.stride + place, have, full, x);
         else
-            sc_route_read<F16, EPL>(a.x, at, have, x);
+            sc_route_read<F16, EPL>(a.x, row * a.stride + place, have, full, x);
         // rows without an order: NaN anywhere, +inf under a softmax
         bool bad = false;
         const int none = a.sigmoid ? 0x003 : 0x203;
 #pragma unroll
         for (int j = 0; j < EPL; ++j) bad |= __builtin_amdgcn_classf(x[j], none);
-        bad = (__ballot(bad) >> first & (L == 64 ? ~0ull : (1ull << L) - 1)) != 0;
+        bad = (__ballot(bad) & row_lanes) != 0;
 
         float m = 0, total = 0, tol = 0;
-        if (want_p) {
+        if (!a.sigmoid && (CLOSE || !a.renorm)) {
+            m = sc_lanes(sc_max<EPL>(x, -INFINITY), L, FMaxOp());
+            m = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+            for (int j = 0; j < EPL; ++j) {
+                s[j] = __builtin_amdgcn_exp2f((x[j] - m) * SC_LOG2E);
+                total += s[j];
+            }
+            total = sc_lanes(total, L, SumOp());
+        }
+        bool again = false, kept = true;
+        if constexpr (CLOSE) {
             if (a.sigmoid) {
 #pragma unroll
                 for (int j = 0; j < EPL; ++j) s[j] = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-SC_LOG2E * x[j]));
-                // error of p: p (1 - p) (|x| u ..) from the exponent, a step each for the exponential, the sum and
-                // the reciprocal, below 4 u; of a difference twice that (u = 2^-24)
+                // p is off by p (1 - p) times the exponent's and the exponential's error and a step each for the sum and
+                // the reciprocal, together below 4 u (u = 2^-24); the difference of two by twice that
                 tol = 0x1p-21f;
             } else {
-                m = sc_lanes(sc_max<EPL>(x, -INFINITY), L, FMaxOp());
-                const float base = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-                for (int j = 0; j < EPL; ++j) {
-                    s[j] = __builtin_amdgcn_exp2f((x[j] - base) * SC_LOG2E);
-                    total += s[j];
-                }
-                total = sc_lanes(total, L, SumOp());
                 const float inv = total == 0 ? 0.0f : 1.0f / total;
 #pragma unroll
                 for (int j = 0; j < EPL; ++j) s[j] *= inv;
-                // the largest p is 1 / total; every p is off by at most (EPL + 30) u of it: the sum's EPL + 6 steps,
-                // the exponents' |t| 2^t, the exponential, the division; of a difference twice that
+                // the largest p is 1 / total, and every p is off by at most (EPL + 40) u of it: the sum's EPL + 6 steps, the
+                // exponents' |t| 2^t, the exponential, the division; the difference of two by twice that
                 tol = 0x1p-17f * inv;
             }
-        }
-        if constexpr (BIAS) {
 #pragma unroll
             for (int j = 0; j < EPL; ++j) s[j] += bias[j];
         }
-        bool again = false, kept = true;
         if (a.groups > 1) {
             float b1 = -INFINITY, b2 = -INFINITY;
 #pragma unroll
             for (int j = 0; j < EPL; ++j) {
-                const float v = j < have ? (by_p ? s[j] : x[j]) : -INFINITY;
+                const float v = j < have ? (CLOSE ? s[j] : x[j]) : -INFINITY;
                 b2 = fmaxf(b2, fminf(b1, v));
                 b1 = fmaxf(b1, v);
             }
-#define SC_TOP2_STEP(d)                                                 \
-    if (a.group_lanes > d) {                                            \
-        const float o1 = sc_across<d>(b1), o2 = sc_across<d>(b2);       \
-        b2 = fmaxf(fminf(b1, o1), fmaxf(b2, o2));                       \
-        b1 = fmaxf(b1, o1);                                             \
+#define SC_TOP2_STEP(d)                                 \
+    if (a.group_lanes > d) {                            \
+        float p1, q1, p2, q2;                           \
+        sc_pair<d>(b1, p1, q1);                         \
+        sc_pair<d>(b2, p2, q2);                         \
+        b2 = fmaxf(fminf(p1, q1), fmaxf(p2, q2));       \
+        b1 = fmaxf(p1, q1);                             \
     }
             SC_TOP2_STEP(1) SC_TOP2_STEP(2) SC_TOP2_STEP(4) SC_TOP2_STEP(8) SC_TOP2_STEP(16) SC_TOP2_STEP(32)
 #undef SC_TOP2_STEP
             const float mine = a.top2 && a.per_group > 1 ? b1 + b2 : b1;
-            if (by_p) {
+            if constexpr (CLOSE) {
                 const float off = 2 * tol + 0x1p-21f * fabsf(mine);
                 int above = 0, maybe = 0;
                 for (int k = 0; k < a.groups; ++k) {
@@ -1122,15 +1175,18 @@ __global__ __launch_bounds__(SC_WG) void k_route(RouteArgs a) {
                 kept = rank < a.top_groups;
             }
         }
-        double best[KP];
+        K best[KP];
         {
             constexpr int B = KP < EPL ? KP : EPL;
 #pragma unroll
             for (int b = 0; b < EPL; b += B) {
-                double v[B];
+                K v[B];
 #pragma unroll
-                for (int j = 0; j < B; ++j)
-                    v[j] = kept && b + j < have ? sc_route_key(BIAS ? s[b + j] : x[b + j], place + b + j) : -INFINITY;
+                for (int j = 0; j < B; ++j) v[j] = Key::make(CLOSE && biased ? s[b + j] : x[b + j], place + b + j);
+                if (!full) {
+#pragma unroll
+                    for (int j = 0; j < B; ++j) v[j] = b + j < have ? v[j] : -INFINITY;
+                }
                 sc_sort<B>(v);
                 if (b == 0) {
 #pragma unroll
@@ -1140,6 +1196,10 @@ __global__ __launch_bounds__(SC_WG) void k_route(RouteArgs a) {
                 }
             }
         }
+        if (a.groups > 1) {
+#pragma unroll
+            for (int j = 0; j < KP; ++j) best[j] = kept ? best[j] : -INFINITY;
+        }
         if (L > 1) sc_merge_across<KP, 1>(best);
         if (L > 2) sc_merge_across<KP, 2>(best);
         if (L > 4) sc_merge_across<KP, 4>(best);
@@ -1147,48 +1207,53 @@ __global__ __launch_bounds__(SC_WG) void k_route(RouteArgs a) {
         if (L > 16) sc_merge_across<KP, 16>(best);
         if (L > 32) sc_merge_across<KP, 32>(best);
 
-        double mine = best[0], last = best[0];
+        K mine = best[0];
 #pragma unroll
-        for (int k = 1; k < KP; ++k) {
-            mine = l == k ? best[k] : mine;
-            last = a.top - 1 == k ? best[k] : last;
-        }
-        if constexpr (BIAS) {
-            // Two neighbours in the list that are too close: in order if they are equal by logit and bias.
-            uint32_t close = 0;
+        for (int k = 1; k < KP; ++k) mine = l == k ? best[k] : mine;
+        const int idx = bad ? -1 : Key::place(mine);
+        if constexpr (!CLOSE) {
+            sc_route_put(a, r, l, L, on, idx, Key::score(mine), m, total);
+        } else {
+            if (biased) {
+                // Two neighbours in the list that are too close: in order if they are equal by logit and bias.
+                K last = best[0];
+                uint32_t close = 0;
 #pragma unroll
-            for (int k = 0; k + 1 < KP; ++k)
-                if (k + 1 < a.top && !(best[k] - best[k + 1] > tol + 0x1p-22 * fabs(best[k]))) close |= 1u << k;
-            if (on && !bad && close) {
+                for (int k = 0; k + 1 < KP; ++k) {
+                    if (k + 1 < a.top && !(best[k] - best[k + 1] > tol + 0x1p-22 * fabs(best[k]))) close |= 1u << k;
+                    last = k + 1 == a.top - 1 ? best[k + 1] : last;
+                }
+                if (on && !bad && close) {
 #pragma unroll
-                for (int k = 0; k + 1 < KP; ++k)
-                    if (close >> k & 1) {
-                        const int p0 = sc_route_place(best[k]), p1 = sc_route_place(best[k + 1]);
-                        again |= sc_logit(a.x, a.dtype, r * a.stride + p0) != sc_logit(a.x, a.dtype, r * a.stride + p1) ||
-                                 a.bias[p0] != a.bias[p1];
-                    }
+                    for (int k = 0; k + 1 < KP; ++k)
+                        if (close >> k & 1) {
+                            const int p0 = Key::place(best[k]), p1 = Key::place(best[k + 1]);
+                            again |= sc_logit(a.x, a.dtype, row * a.stride + p0) != sc_logit(a.x, a.dtype, row * a.stride + p1) ||
+                                     a.bias[p0] != a.bias[p1];
+                        }
+                }
+                // An expert too close to the last one chosen, on either side: the choice stands if they are equal.
+                const float edge = (float)last, off = tol + 0x1p-22f * fabsf(edge);
+                const int pl = Key::place(last);
+                bool near = false;
+#pragma unroll
+                for (int j = 0; j < EPL; ++j) near |= !(fabsf(s[j] - edge) > off) && place + j != pl;
+                if (on && !bad && near && kept) {
+                    const float xl = sc_logit(a.x, a.dtype, row * a.stride + pl), bl = a.bias[pl];
+#pragma unroll
+                    for (int j = 0; j < EPL; ++j)
+                        again |= j < have && !(fabsf(s[j] - edge) > off) && place + j != pl && (x[j] != xl || bias[j] != bl);
+                }
             }
-            // An expert too close to the last one chosen, on either side: the choice stands if they are equal.
-            const float edge = (float)last, off = tol + 0x1p-22f * fabsf(edge);
-            bool near = false;
-#pragma unroll
-            for (int j = 0; j < EPL; ++j) near |= j < have && kept && !(fabsf(s[j] - edge) > off);
-            if (on && !bad && near) {
-                const int pl = sc_route_place(last);
-                const float xl = sc_logit(a.x, a.dtype, r * a.stride + pl), bl = a.bias[pl];
-#pragma unroll
-                for (int j = 0; j < EPL; ++j)
-                    again |= j < have && !(fabsf(s[j] - edge) > off) && place + j != pl && (x[j] != xl || bias[j] != bl);
+            uint64_t todo = __ballot(again && on && !bad);
+            const bool put = on && !(todo & row_lanes);
+            const float xi = put && l < a.top && idx >= 0 ? sc_logit(a.x, a.dtype, row * a.stride + idx) : -INFINITY;
+            sc_route_put(a, r, l, L, put, idx, xi, m, total);
+            while (todo) {  // rows whose order float32 does not tell: here, where the sorting's registers are free again
+                const int from = (__ffsll((unsigned long long)todo) - 1) & ~(L - 1);
+                sc_route_row(a, tile * per_wave + from / L, lane, by[wave]);
+                todo &= ~((L == 64 ? ~0ull : (1ull << L) - 1) << from);
             }
-        }
-        uint64_t todo = __ballot(again && on && !bad);
-        const uint64_t row_lanes = L == 64 ? ~0ull : (1ull << L) - 1;
-        const bool put = on && !(todo >> first & row_lanes);
-        sc_route_put(a, r, l, L, put, bad ? -1 : sc_route_place(mine), m == -INFINITY ? 0.0f : m, total);
-        while (todo) {  // rows whose order float32 does not tell: here, where the sorting's registers are free again
-            const int from = (__ffsll((unsigned long long)todo) - 1) & ~(L - 1);
-            sc_route_row(a, tile * per_wave + from / L, lane);
-            todo &= ~(row_lanes << from);
         }
     }
 }
@@ -1435,37 +1500,39 @@ static int sc_check_route(const char* fn, int64_t experts, int top, int score) {
     return 0;
 }
 
+#define SC_ROUTE_WAVES 2048
+
 static int sc_pow2(int v) {
     int p = 1;
     while (p < v) p *= 2;
     return p;
 }
 
-template <int EPL, bool BIAS>
+template <int EPL, int MODE>
 static void sc_launch_route_epl(const RouteArgs& a, int kp, unsigned grid, hipStream_t stream) {
     const dim3 wg(SC_WG);
     if (kp == 2)
-        hipLaunchKernelGGL((k_route<EPL, 2, BIAS>), dim3(grid), wg, 0, stream, a);
+        hipLaunchKernelGGL((k_route<EPL, 2, MODE>), dim3(grid), wg, 0, stream, a);
     else if (kp == 4)
-        hipLaunchKernelGGL((k_route<EPL, 4, BIAS>), dim3(grid), wg, 0, stream, a);
+        hipLaunchKernelGGL((k_route<EPL, 4, MODE>), dim3(grid), wg, 0, stream, a);
     else if (kp == 8)
-        hipLaunchKernelGGL((k_route<EPL, 8, BIAS>), dim3(grid), wg, 0, stream, a);
+        hipLaunchKernelGGL((k_route<EPL, 8, MODE>), dim3(grid), wg, 0, stream, a);
     else if (kp == 16)
-        hipLaunchKernelGGL((k_route<EPL, 16, BIAS>), dim3(grid), wg, 0, stream, a);
+        hipLaunchKernelGGL((k_route<EPL, 16, MODE>), dim3(grid), wg, 0, stream, a);
     else
-        hipLaunchKernelGGL((k_route<EPL, 32, BIAS>), dim3(grid), wg, 0, stream, a);
+        hipLaunchKernelGGL((k_route<EPL, 32, MODE>), dim3(grid), wg, 0, stream, a);
 }
 
-template <bool BIAS>
+template <int MODE>
 static void sc_launch_route(const RouteArgs& a, int epl, int kp, hipStream_t stream) {
     const int64_t rows_wg = 64 / a.lanes * SC_WAVES;
     const unsigned grid = sc_grid((a.rows + rows_wg - 1) / rows_wg);
     if (epl <= 8)
-        sc_launch_route_epl<8, BIAS>(a, kp, grid, stream);
+        sc_launch_route_epl<8, MODE>(a, kp, grid, stream);
     else if (epl <= 16)
-        sc_launch_route_epl<16, BIAS>(a, kp, grid, stream);
+        sc_launch_route_epl<16, MODE>(a, kp, grid, stream);
     else
-        sc_launch_route_epl<32, BIAS>(a, kp, grid, stream);
+        sc_launch_route_epl<32, MODE>(a, kp, grid, stream);
 }
 
 extern "C" int pd_route_experts(const void* logits, int dtype, int64_t rows, int64_t experts, int64_t row_stride,
@@ -1483,17 +1550,21 @@ extern "C" int pd_route_experts(const void* logits, int dtype, int64_t rows, int
     if (!weights || !index) return sc_fail(fn, "weights and index are required");
     RouteArgs a = {logits, dtype, rows, row_stride, (int)experts, top, score == PD_SCORE_SIGMOID, bias, groups, (int)experts / groups,
                    top_groups, group_score == PD_GROUP_TOP2, renormalise != 0, scale, weights, index};
-    // The fewest lanes that hold a row (at most 32 experts each), a group each at least, and write its `top` results:
-    // a lane's work grows more slowly with its experts than the number of rows in a wavefront falls with its lanes.
+    // The fewest lanes that hold a row, 16 experts each at most: a lane's work grows more slowly with its experts than the
+    // rows of a wavefront fall with its lanes.  Where the rows leave most of the chip idle anyway a lane takes 8; 32 where
+    // an odd number of groups would take more than the 64 lanes (G > gp / 2 groups of at most 1024 / G always fit then).
     const int kp = sc_pow2(top < 2 ? 2 : top), gp = sc_pow2(groups);
     a.lanes = kp > gp ? kp : gp;
-    while (a.lanes / gp * 32 < a.per_group) a.lanes *= 2;
+    while (a.lanes < 64 && a.lanes / gp * 16 < a.per_group) a.lanes *= 2;
+    if (a.lanes < 64 && a.lanes / gp * 8 < a.per_group && rows * a.lanes < 64 * SC_ROUTE_WAVES) a.lanes *= 2;
     a.group_lanes = a.lanes / gp;
     const int epl = (a.per_group + a.group_lanes - 1) / a.group_lanes;
-    if (bias)
-        sc_launch_route<true>(a, epl, kp, (hipStream_t)stream);
+    if (bias || (groups > 1 && a.top2))
+        sc_launch_route<ROUTE_CLOSE>(a, epl, kp, (hipStream_t)stream);
+    else if (dtype == PD_F32)
+        sc_launch_route<ROUTE_PLAIN32>(a, epl, kp, (hipStream_t)stream);
     else
-        sc_launch_route<false>(a, epl, kp, (hipStream_t)stream);
+        sc_launch_route<ROUTE_PLAIN16>(a, epl, kp, (hipStream_t)stream);
     return sc_launched(fn);
 }
 
