@@ -186,16 +186,27 @@ __device__ __forceinline__ T sc_wave(T v, F f) {
     return sc_lanes(v, 64, f);
 }
 
-template <typename T, typename F>
-__device__ T sc_block(T v, F f, T* lds) {  // lds: SC_WAVES values
+template <int WG, typename T, typename F>
+__device__ T sc_block(T v, F f, T* lds) {  // lds: WG / 64 values
     v = sc_wave(v, f);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
     __syncthreads();
     v = lds[0];
 #pragma unroll
-    for (int i = 1; i < SC_WAVES; ++i) v = f(v, lds[i]);
+    for (int i = 1; i < WG / 64; ++i) v = f(v, lds[i]);
     return v;
+}
+
+// How many of the n keys (in LDS, n <= the room there) are larger.
+__device__ __forceinline__ int sc_rank(const uint64_t* keys, int n, uint64_t key) {
+    int rank = 0, j = 0;
+    for (; j + 8 <= n; j += 8) {  // eight reads in flight
+#pragma unroll
+        for (int i = 0; i < 8; ++i) rank += keys[j + i] > key;
+    }
+    for (; j < n; ++j) rank += keys[j] > key;
+    return rank;
 }
 
 // ---- log probabilities ---------------------------------------------------------------------
@@ -252,6 +263,26 @@ __device__ __forceinline__ void sc_join_wave(Stat& st) {
     sc_carry(st, sc_wave(st.m, FMaxOp()));
     st.s = sc_wave(st.s, SumOp());
     st.w = sc_wave(st.w, SumOp());
+}
+
+// The same over a workgroup; every thread gets it.  The caller synchronises before wave_stat is used again.
+template <int WG>
+__device__ __forceinline__ void sc_join_block(Stat& st, Stat* wave_stat) {
+    sc_join_wave(st);
+    if ((threadIdx.x & 63) == 0) wave_stat[threadIdx.x >> 6] = st;
+    __syncthreads();
+    float m = wave_stat[0].m;
+#pragma unroll
+    for (int i = 1; i < WG / 64; ++i) m = fmaxf(m, wave_stat[i].m);
+    st = wave_stat[0];
+    sc_carry(st, m);
+#pragma unroll
+    for (int i = 1; i < WG / 64; ++i) {
+        Stat o = wave_stat[i];
+        sc_carry(o, m);
+        st.s += o.s;
+        st.w += o.w;
+    }
 }
 
 struct RowStat {
@@ -386,8 +417,7 @@ __global__ __launch_bounds__(SC_WG) void k_token_logprobs_wave(LogprobArgs a) {
         if (count <= SC_WAVE_CAND) {
             for (int i = lane; i < count; i += 64) {
                 const uint64_t key = mine[i];
-                int rank = 0;
-                for (int j = 0; j < count; ++j) rank += mine[j] > key;
+                const int rank = sc_rank(mine, count, key);
                 if (rank < a.top) sc_put_top(a, r, rank, key, q);
             }
             if (lane >= count && lane < a.top) sc_put_top(a, r, lane, 0, q);
@@ -411,47 +441,48 @@ __global__ __launch_bounds__(SC_WG) void k_token_logprobs_wave(LogprobArgs a) {
 
 // ---- a workgroup to the row, or to a slice of it ------------------------------------------------
 //
-// Chunks of 8192 columns, 32 to a thread in 16-byte loads; eight workgroups to a CU keep the loads coming while
-// others reduce.  Bound by the memory where there are rows enough.  A row is cut into slices of whole chunks where
-// rows alone do not fill the chip, or where it is longer than SC_MAX_CHUNKS chunks; the slices are joined by
-// k_token_logprobs_join.
+// Chunks of WG * 32 columns, 32 to a thread in 16-byte loads.  With many rows: 256 threads, six to eight workgroups
+// to a CU keep the loads coming while others reduce; bound by the memory (4096 x 131072 bfloat16 with five alternatives:
+// 199 us, 5.4 TB/s).  With fewer rows than CUs: 1024 threads that load a chunk while they add the one before; bound by
+// what one CU can have in flight, and by the latency of the steps behind the last load.  Rows that would take one CU long
+// are cut into slices, joined by k_token_logprobs_join.
 
 #define SC_PER_THREAD 32
-#define SC_CHUNK (SC_WG * SC_PER_THREAD)
-#define SC_MAX_CHUNKS 16
+#define SC_MAX_CHUNKS(WG) ((WG) == 1024 ? 8 : 16)
 #define SC_SEGS 128   // segments that are read again
 #define SC_CAND 512   // candidates that are put into order
 
+template <int WG>
 struct TopShared {
-    uint32_t seg_max[SC_MAX_CHUNKS][SC_WG];
-    uint32_t lane_max[SC_WG];
+    uint32_t seg_max[SC_MAX_CHUNKS(WG)][WG];
+    uint32_t part_max[256];
     uint64_t cand[SC_CAND];
-    uint64_t wave_best[SC_WAVES];
+    uint64_t wave_best[WG / 64];
     uint16_t segs[SC_SEGS];
     uint32_t tau;
-    int n_seg, n_cand, scanned[SC_WAVES];
+    int n_seg, n_cand, scanned[WG / 64];
 };
 
 // Reads the segments whose maximum is at least `from` again and collects their scores from there on (orders).
 // False: there are more of either than there is room for.
-template <typename X>
-__device__ bool sc_collect(TopShared& sh, const typename X::E* x, int begin, int end, uint32_t from) {
-    constexpr int V = X::V, NV = SC_PER_THREAD / V;
+template <typename X, int WG>
+__device__ bool sc_collect(TopShared<WG>& sh, const typename X::E* x, int begin, int end, uint32_t from) {
+    constexpr int V = X::V, NV = SC_PER_THREAD / V, CHUNK = WG * SC_PER_THREAD;
     const int t = threadIdx.x;
     __syncthreads();
     if (t == 0) sh.n_seg = sh.n_cand = 0;
     __syncthreads();
-    const int chunks = (end - begin + SC_CHUNK - 1) / SC_CHUNK;
+    const int chunks = (end - begin + CHUNK - 1) / CHUNK;
     for (int c = 0; c < chunks; ++c)
         if (sh.seg_max[c][t] >= from) {
             const int to = atomicAdd(&sh.n_seg, 1);
-            if (to < SC_SEGS) sh.segs[to] = (uint16_t)(c * SC_WG + t);
+            if (to < SC_SEGS) sh.segs[to] = (uint16_t)(c * WG + t);
         }
     __syncthreads();
     if (sh.n_seg > SC_SEGS) return false;
-    for (int i = t; i < sh.n_seg * NV; i += SC_WG) {
+    for (int i = t; i < sh.n_seg * NV; i += WG) {
         const int seg = sh.segs[i / NV];
-        const int at = begin + (seg / SC_WG) * SC_CHUNK + ((i % NV) * SC_WG + seg % SC_WG) * V;
+        const int at = begin + (seg / WG) * CHUNK + ((i % NV) * WG + seg % WG) * V;
         if (at >= end) continue;
         float f[V];
         sc_read<X>(x, at, end, f);
@@ -468,27 +499,33 @@ __device__ bool sc_collect(TopShared& sh, const typename X::E* x, int begin, int
 
 // The `top` largest of columns begin .. end - 1 as keys, put(k, key) called once for each k, with 0 where there
 // are no more columns.  lane_max: the largest of this thread's columns.  The segments' maxima are in sh.
-template <typename X, typename Put>
-__device__ void sc_top_block(TopShared& sh, const typename X::E* x, int begin, int end, int top, float lane_max, Put put) {
+template <typename X, int WG, typename Put>
+__device__ void sc_top_block(TopShared<WG>& sh, const typename X::E* x, int begin, int end, int top, float lane_max, Put put) {
     constexpr int V = X::V;
     const int t = threadIdx.x;
-    sh.lane_max[t] = sc_order(lane_max);
+    // 256 parts of the columns, a thread's or four threads': the top-th largest of their maxima (top <= 64) is a bound
+    if constexpr (WG == 1024) {
+        lane_max = sc_lanes(lane_max, 4, FMaxOp());
+        if ((t & 3) == 0) sh.part_max[t / 4] = sc_order(lane_max);
+    } else {
+        sh.part_max[t] = sc_order(lane_max);
+    }
     __syncthreads();
     if (t < 64) {
-        uint32_t o[SC_WAVES];
+        uint32_t o[4];
 #pragma unroll
-        for (int i = 0; i < SC_WAVES; ++i) o[i] = sh.lane_max[t + 64 * i];
-        const uint32_t tau = sc_kth<SC_WAVES>(o, top);
+        for (int i = 0; i < 4; ++i) o[i] = sh.part_max[t + 64 * i];
+        const uint32_t tau = sc_kth<4>(o, top);
         if (t == 0) sh.tau = tau;
     }
     __syncthreads();
     const uint32_t tau = sh.tau;
-    bool fits = sc_collect<X>(sh, x, begin, end, tau);
-    if (!fits && sc_collect<X>(sh, x, begin, end, tau + 1)) {
+    bool fits = sc_collect<X, WG>(sh, x, begin, end, tau);
+    if (!fits && sc_collect<X, WG>(sh, x, begin, end, tau + 1)) {
         // too many scores equal to tau (a masked row, a constant one): what is larger has been collected, and the
         // first of the equal ones make up the number, found from the front
         fits = true;
-        for (int at0 = begin; at0 < end && sh.n_cand < top; at0 += SC_WG * V) {
+        for (int at0 = begin; at0 < end && sh.n_cand < top; at0 += WG * V) {
             const int at = at0 + t * V;
             float f[V];
             sc_read<X>(x, at, end, f);
@@ -507,7 +544,7 @@ __device__ void sc_top_block(TopShared& sh, const typename X::E* x, int begin, i
             int total = 0;
             before += have - mine;
 #pragma unroll
-            for (int i = 0; i < SC_WAVES; ++i) {
+            for (int i = 0; i < WG / 64; ++i) {
                 if (i < t >> 6) before += sh.scanned[i];
                 total += sh.scanned[i];
             }
@@ -523,10 +560,9 @@ __device__ void sc_top_block(TopShared& sh, const typename X::E* x, int begin, i
     }
     if (fits) {
         const int n = sh.n_cand;
-        for (int i = t; i < n; i += SC_WG) {
+        for (int i = t; i < n; i += WG) {
             const uint64_t key = sh.cand[i];
-            int rank = 0;
-            for (int j = 0; j < n; ++j) rank += sh.cand[j] > key;
+            const int rank = sc_rank(sh.cand, n, key);
             if (rank < top) put(rank, key);
         }
         if (t >= n && t < top) put(t, 0);
@@ -534,7 +570,7 @@ __device__ void sc_top_block(TopShared& sh, const typename X::E* x, int begin, i
         uint64_t prev = ~0ull;  // many large scores in few lanes: one after the other
         for (int k = 0; k < top; ++k) {
             uint64_t best = 0;
-            for (int at = begin + t * V; at < end; at += SC_WG * V) {
+            for (int at = begin + t * V; at < end; at += WG * V) {
                 float f[V];
                 sc_read<X>(x, at, end, f);
 #pragma unroll
@@ -543,20 +579,28 @@ __device__ void sc_top_block(TopShared& sh, const typename X::E* x, int begin, i
                     if (at + e < end && key < prev && key > best) best = key;
                 }
             }
-            prev = sc_block(best, MaxOp(), sh.wave_best);
+            prev = sc_block<WG>(best, MaxOp(), sh.wave_best);
             if (t == 0) put(k, prev);
         }
     }
     __syncthreads();
 }
 
+// Thread t's 32 scores of a whole chunk that starts at x.
+template <typename X, int WG>
+__device__ __forceinline__ void sc_load_chunk(const typename X::E* x, int t, sc_u4* w) {
+#pragma unroll
+    for (int u = 0; u < SC_PER_THREAD / X::V; ++u) w[u] = sc_load<X>(x + (u * WG + t) * X::V);
+}
+
 struct Nothing {};
 
-template <typename X, bool TOP>
-__global__ __launch_bounds__(SC_WG) void k_token_logprobs_block(LogprobArgs a) {
-    constexpr int V = X::V, NV = SC_PER_THREAD / V;
-    __shared__ Stat wave_stat[SC_WAVES];
-    __shared__ typename std::conditional<TOP, TopShared, Nothing>::type sh;
+template <typename X, int WG, bool TOP>
+__global__ __launch_bounds__(WG) void k_token_logprobs_block(LogprobArgs a) {
+    constexpr int V = X::V, NV = SC_PER_THREAD / V, CHUNK = WG * SC_PER_THREAD, WAVES = WG / 64;
+    constexpr bool AHEAD = WG == 1024;  // few workgroups: nobody else to fill the time between a load and its use
+    __shared__ Stat wave_stat[WAVES];
+    __shared__ typename std::conditional<TOP, TopShared<WG>, Nothing>::type sh;
     const int t = threadIdx.x;
     for (int64_t b = blockIdx.x; b < a.rows * a.slices; b += gridDim.x) {
         const int64_t r = b / a.slices;
@@ -566,17 +610,18 @@ __global__ __launch_bounds__(SC_WG) void k_token_logprobs_block(LogprobArgs a) {
         const int begin = slice * a.slice_cols < n ? slice * a.slice_cols : n;
         const int end = n - begin < a.slice_cols ? n : begin + a.slice_cols;
         Stat st = {-INFINITY, 0, 0};
-        for (int c = 0, at0 = begin; at0 < end; at0 += SC_CHUNK, ++c) {
+        sc_u4 w[NV];
+        if (AHEAD && begin + CHUNK <= end) sc_load_chunk<X, WG>(x + begin, t, w);
+        for (int c = 0, at0 = begin; at0 < end; at0 += CHUNK, ++c) {
             float f[SC_PER_THREAD];
-            if (at0 + SC_CHUNK <= end) {
-                sc_u4 w[NV];
-#pragma unroll
-                for (int u = 0; u < NV; ++u) w[u] = sc_load<X>(x + at0 + (u * SC_WG + t) * V);
+            if (at0 + CHUNK <= end) {
+                if (!AHEAD) sc_load_chunk<X, WG>(x + at0, t, w);
 #pragma unroll
                 for (int u = 0; u < NV; ++u) X::unpack(w[u], f + u * V);
+                if (AHEAD && at0 + 2 * CHUNK <= end) sc_load_chunk<X, WG>(x + at0 + CHUNK, t, w);
             } else {
 #pragma unroll
-                for (int u = 0; u < NV; ++u) sc_read<X>(x, at0 + (u * SC_WG + t) * V, end, f + u * V);
+                for (int u = 0; u < NV; ++u) sc_read<X>(x, at0 + (u * WG + t) * V, end, f + u * V);
             }
             const float m = sc_max<SC_PER_THREAD>(f, -INFINITY);
             if constexpr (TOP) sh.seg_max[c][t] = sc_order(m);
@@ -584,24 +629,12 @@ __global__ __launch_bounds__(SC_WG) void k_token_logprobs_block(LogprobArgs a) {
             sc_add<SC_PER_THREAD>(st, f);
         }
         const float lane_max = st.m;
-        sc_join_wave(st);
-        if ((t & 63) == 0) wave_stat[t >> 6] = st;
-        __syncthreads();
-        st = wave_stat[0];
-#pragma unroll
-        for (int i = 1; i < SC_WAVES; ++i) {
-            Stat o = wave_stat[i];
-            const float m = fmaxf(st.m, o.m);
-            sc_carry(st, m);
-            sc_carry(o, m);
-            st.s += o.s;
-            st.w += o.w;
-        }
+        sc_join_block<WG>(st, wave_stat);
         const RowStat q = sc_row_stat(st);
         if (a.slices > 1) {
             if (t == 0) a.part[b] = st;
         } else {
-            sc_put_row<X>(a, r, x, n, st, q, t, SC_WG);
+            sc_put_row<X>(a, r, x, n, st, q, t, WG);
         }
         if constexpr (TOP) {
             if (a.slices > 1) {
@@ -609,12 +642,12 @@ __global__ __launch_bounds__(SC_WG) void k_token_logprobs_block(LogprobArgs a) {
                 if (q.bad) {
                     if (t < a.top) keys[t] = 0;
                 } else {
-                    sc_top_block<X>(sh, x, begin, end, a.top, lane_max, [&](int k, uint64_t key) { keys[k] = key; });
+                    sc_top_block<X, WG>(sh, x, begin, end, a.top, lane_max, [&](int k, uint64_t key) { keys[k] = key; });
                 }
             } else if (q.bad || q.empty) {
                 if (t < a.top) sc_put_top(a, r, t, q.bad ? 0 : sc_key(-INFINITY, t), q);
             } else {
-                sc_top_block<X>(sh, x, begin, end, a.top, lane_max, [&](int k, uint64_t key) { sc_put_top(a, r, k, key, q); });
+                sc_top_block<X, WG>(sh, x, begin, end, a.top, lane_max, [&](int k, uint64_t key) { sc_put_top(a, r, k, key, q); });
             }
         }
         __syncthreads();  // wave_stat is written again
@@ -641,20 +674,8 @@ __global__ __launch_bounds__(SC_WG) void k_token_logprobs_join(LogprobArgs a) {
             st.s += o.s;
             st.w += o.w;
         }
-        sc_join_wave(st);
         if (t == 0) n_cand = 0;
-        if ((t & 63) == 0) wave_stat[t >> 6] = st;
-        __syncthreads();
-        st = wave_stat[0];
-#pragma unroll
-        for (int i = 1; i < SC_WAVES; ++i) {
-            Stat o = wave_stat[i];
-            const float m = fmaxf(st.m, o.m);
-            sc_carry(st, m);
-            sc_carry(o, m);
-            st.s += o.s;
-            st.w += o.w;
-        }
+        sc_join_block<SC_WG>(st, wave_stat);
         const RowStat q = sc_row_stat(st);
         sc_put_row<X>(a, r, x, n, st, q, t, SC_WG);
         if (a.top && (q.bad || q.empty)) {
@@ -664,7 +685,7 @@ __global__ __launch_bounds__(SC_WG) void k_token_logprobs_join(LogprobArgs a) {
             const int total = a.slices * a.top, j = (a.top + a.slices - 1) / a.slices;
             uint64_t from = ~0ull;
             for (int i = t; i < a.slices; i += SC_WG) from = MinOp()(from, keys[i * a.top + j - 1]);
-            from = sc_block(from, MinOp(), wave_key);
+            from = sc_block<SC_WG>(from, MinOp(), wave_key);
             for (int i = t; i < total; i += SC_WG) {
                 const uint64_t key = keys[i];
                 if (key && key >= from) {
@@ -677,8 +698,7 @@ __global__ __launch_bounds__(SC_WG) void k_token_logprobs_join(LogprobArgs a) {
             if (have <= SC_CAND) {
                 for (int i = t; i < have; i += SC_WG) {
                     const uint64_t key = cand[i];
-                    int rank = 0;
-                    for (int k = 0; k < have; ++k) rank += cand[k] > key;
+                    const int rank = sc_rank(cand, have, key);
                     if (rank < a.top) sc_put_top(a, r, rank, key, q);
                 }
                 if (t >= have && t < a.top) sc_put_top(a, r, t, 0, q);
@@ -688,7 +708,7 @@ __global__ __launch_bounds__(SC_WG) void k_token_logprobs_join(LogprobArgs a) {
                     uint64_t best = 0;
                     for (int i = t; i < total; i += SC_WG)
                         if (keys[i] < prev && keys[i] > best) best = keys[i];
-                    prev = sc_block(best, MaxOp(), wave_key);
+                    prev = sc_block<SC_WG>(best, MaxOp(), wave_key);
                     if (t == 0) sc_put_top(a, r, k, prev, q);
                 }
             }
@@ -792,6 +812,8 @@ __global__ __launch_bounds__(SC_WG) void k_token_logprobs_grad_wave(LogprobGradA
         for (int u = 0; u < NV; ++u) sc_grad_store<X>(out, (u * 64 + lane) * V, n, a.cols, q.empty, f + u * V);
     }
 }
+
+#define SC_CHUNK (SC_WG * SC_PER_THREAD)
 
 template <typename X>
 __global__ __launch_bounds__(SC_WG) void k_token_logprobs_grad_block(LogprobGradArgs a) {
@@ -1368,34 +1390,52 @@ static int sc_check_grad(const char* fn, const void* x, int dtype, int64_t rows,
             hipLaunchKernelGGL((kernel<F16>), dim3(grid), dim3(SC_WG), 0, (hipStream_t)(stream), args);   \
     } while (0)
 
-// How a call with a workgroup to the row is cut.  The chip runs some 2000 workgroups at a time; with fewer rows than
-// SC_FILL a row is cut into more slices, of whole chunks.
+// How a call with a workgroup to the row is cut: 256 threads a row where there are rows for every CU, 1024 with fewer; the
+// latter in slices of at least SC_SLICE_BYTES, as many as there are CUs for, which is what one CU reads in the time
+// that the join costs.
 #define SC_WAVE_COLS 2048
-#define SC_FILL 512
+#define SC_CUS 256
+#define SC_SLICE_BYTES (512 << 10)
 
-static void sc_slices(int64_t rows, int64_t cols, int* slices, int* slice_cols) {
-    const int64_t chunks = (cols + SC_CHUNK - 1) / SC_CHUNK;
-    int64_t want = rows >= SC_FILL ? 1 : SC_FILL / rows;
-    const int64_t least = (chunks + SC_MAX_CHUNKS - 1) / SC_MAX_CHUNKS;
+struct Cut {
+    int wg, slices, slice_cols;
+};
+
+static Cut sc_cut(int dtype, int64_t rows, int64_t cols) {
+    Cut c;
+    c.wg = rows >= SC_CUS ? SC_WG : 1024;
+    const int64_t chunk = (int64_t)c.wg * SC_PER_THREAD, chunks = (cols + chunk - 1) / chunk;
+    int64_t want = rows >= SC_CUS ? 1 : SC_CUS / rows;
+    const int64_t most = cols * sc_size(dtype) / SC_SLICE_BYTES, least = (chunks + SC_MAX_CHUNKS(c.wg) - 1) / SC_MAX_CHUNKS(c.wg);
+    if (want > most) want = most;
     if (want < least) want = least;
-    if (want > chunks) want = chunks;
     const int64_t each = (chunks + want - 1) / want;
-    *slices = (int)((chunks + each - 1) / each);
-    *slice_cols = (int)each * SC_CHUNK;
+    c.slices = (int)((chunks + each - 1) / each);
+    c.slice_cols = (int)(each * chunk);
+    return c;
 }
 
 extern "C" uint64_t pd_token_logprobs_workspace(int dtype, int64_t rows, int64_t columns, int top) {
     if (!sc_size(dtype) || rows < 1 || rows > INT32_MAX || columns <= SC_WAVE_COLS || columns > PD_MAX_COLUMNS || top < 0 ||
         top > PD_MAX_ALTERNATIVES)
         return 0;
-    int slices, slice_cols;
-    sc_slices(rows, columns, &slices, &slice_cols);
-    if (slices == 1) return 0;
-    return (((uint64_t)rows * slices * sizeof(Stat) + 15) & ~15ull) + (uint64_t)rows * slices * top * sizeof(uint64_t);
+    const Cut c = sc_cut(dtype, rows, columns);
+    if (c.slices == 1) return 0;
+    return (((uint64_t)rows * c.slices * sizeof(Stat) + 15) & ~15ull) + (uint64_t)rows * c.slices * top * sizeof(uint64_t);
+}
+
+template <typename X, int WG>
+static void sc_launch_logprobs_block(const LogprobArgs& a, hipStream_t stream) {
+    const dim3 grid(sc_grid(a.rows * a.slices)), wg(WG);
+    if (a.top)
+        hipLaunchKernelGGL((k_token_logprobs_block<X, WG, true>), grid, wg, 0, stream, a);
+    else
+        hipLaunchKernelGGL((k_token_logprobs_block<X, WG, false>), grid, wg, 0, stream, a);
+    if (a.slices > 1) hipLaunchKernelGGL((k_token_logprobs_join<X>), dim3(sc_grid(a.rows)), dim3(SC_WG), 0, stream, a);
 }
 
 template <typename X>
-static void sc_launch_logprobs(const LogprobArgs& a, hipStream_t stream) {
+static void sc_launch_logprobs(const LogprobArgs& a, int wg_size, hipStream_t stream) {
     const dim3 wg(SC_WG);
     if (a.cols <= SC_WAVE_COLS) {
         const dim3 grid(sc_grid((a.rows + SC_WAVES - 1) / SC_WAVES));
@@ -1410,12 +1450,10 @@ static void sc_launch_logprobs(const LogprobArgs& a, hipStream_t stream) {
             hipLaunchKernelGGL((k_token_logprobs_wave<X, SC_WAVE_COLS / 64 / X::V>), grid, wg, 0, stream, a);
         return;
     }
-    const dim3 grid(sc_grid(a.rows * a.slices));
-    if (a.top)
-        hipLaunchKernelGGL((k_token_logprobs_block<X, true>), grid, wg, 0, stream, a);
+    if (wg_size == SC_WG)
+        sc_launch_logprobs_block<X, SC_WG>(a, stream);
     else
-        hipLaunchKernelGGL((k_token_logprobs_block<X, false>), grid, wg, 0, stream, a);
-    if (a.slices > 1) hipLaunchKernelGGL((k_token_logprobs_join<X>), dim3(sc_grid(a.rows)), wg, 0, stream, a);
+        sc_launch_logprobs_block<X, 1024>(a, stream);
 }
 
 extern "C" int pd_token_logprobs(const void* logits, int dtype, int64_t rows, int64_t columns, int64_t row_stride,
@@ -1437,18 +1475,19 @@ extern "C" int pd_token_logprobs(const void* logits, int dtype, int64_t rows, in
     }
     if (need && ((uintptr_t)workspace & 15)) return sc_fail(fn, "the workspace is not 16-byte aligned");
     LogprobArgs a = {logits, rows, row_stride, (int)columns, widths, tokens, n_tokens, top, logp, entropy, stats, top_logp, top_index};
-    a.slices = 1;
-    if (columns > SC_WAVE_COLS) sc_slices(rows, columns, &a.slices, &a.slice_cols);
+    const Cut cut = sc_cut(dtype, rows, columns);
+    a.slices = cut.slices;
+    a.slice_cols = cut.slice_cols;
     if (need) {
         a.part = (Stat*)workspace;
         a.part_keys = (uint64_t*)((char*)workspace + (((uint64_t)rows * a.slices * sizeof(Stat) + 15) & ~15ull));
     }
     if (dtype == PD_F32)
-        sc_launch_logprobs<F32>(a, (hipStream_t)stream);
+        sc_launch_logprobs<F32>(a, cut.wg, (hipStream_t)stream);
     else if (dtype == PD_BF16)
-        sc_launch_logprobs<BF16>(a, (hipStream_t)stream);
+        sc_launch_logprobs<BF16>(a, cut.wg, (hipStream_t)stream);
     else
-        sc_launch_logprobs<F16>(a, (hipStream_t)stream);
+        sc_launch_logprobs<F16>(a, cut.wg, (hipStream_t)stream);
     return sc_launched(fn);
 }
 

@@ -63,11 +63,13 @@ def _tokens(tokens, rows, device):
 def _call(fn, device, *args):
     """One call of the library on the current stream of ``device``."""
     L = _ffi.lib()
+    # (the stream's address itself: making a Stream object of it takes longer than the rest of a small call's checks)
+    stream = torch._C._cuda_getCurrentRawStream(device.index)
     if torch.cuda.current_device() != device.index:
         with torch.cuda.device(device):
-            rc = getattr(L, fn)(*args, torch.cuda.current_stream().cuda_stream)
+            rc = getattr(L, fn)(*args, stream)
     else:
-        rc = getattr(L, fn)(*args, torch.cuda.current_stream().cuda_stream)
+        rc = getattr(L, fn)(*args, stream)
     if rc == _ffi.PD_OK:
         return
     msg = L.pd_last_error(None).decode()

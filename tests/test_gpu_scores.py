@@ -85,9 +85,31 @@ def _check_logprobs(x, tokens=None, top=0, widths=None):
     return r
 
 
+def _check_many(x, tokens=None, top=0, widths=None, times=19):
+    """The rows of x over and over: a call of many rows, cut differently, against the restatement for the first ones
+    and itself for the others."""
+    one = _check_logprobs(x, tokens, top, widths)
+    rows = x.shape[0]
+
+    def again(v):
+        return None if v is None else v.repeat(times, *[1] * (v.dim() - 1))
+    many = _scores().token_logprobs(again(x), again(tokens), top=top, widths=again(widths))
+    err = (x.shape[1] / 64 + 96) * U * (1 + math.log(x.shape[1] + 1))
+    for a, b in zip(many, one):
+        if a is not None:
+            first = a[:rows]
+            assert torch.equal(a.nan_to_num(nan=7.0), first.repeat(times, *[1] * (a.dim() - 1)).nan_to_num(nan=7.0))
+            if a.dtype == torch.int32:
+                assert torch.equal(first, b)
+            else:
+                _close(first, _np(b), 2 * err + 4 * U * np.abs(np.nan_to_num(_np(b), posinf=0, neginf=0)), 'many rows')
+    return one
+
+
 SHAPES = [(1, 1, 1), (3, 2, 2), (5, 63, 3), (2, 64, 64), (4, 65, 5), (300, 7, 7), (7, 368, 5), (33, 656, 3), (3, 1000, 20),
           (9, 1024, 1), (5, 1025, 9), (2, 2047, 64), (3, 2049, 8), (4, 4099, 0), (2, 8193, 17), (3, 32003, 8), (2, 50021, 33),
-          (1, 131072, 20), (1, 131073, 64), (2, 262149, 5)]
+          (1, 131072, 20), (1, 131073, 64), (2, 262149, 5),
+          (1, 1200001, 7)]
 
 
 @pytest.mark.parametrize('dtype', list(TYPES))
@@ -126,11 +148,12 @@ def test_logprobs_of_masked_infinite_equal_and_nan_rows(cols, dtype):
     x[13, cols // 3] = high
     x[14] = (torch.arange(cols, device='cuda') % 4).to(x.dtype)                          # four values, many ties
     top = min(cols, 40)
-    _check_logprobs(x, _tokens(15, cols, 4, seed=cols), top)
+    _check_many(x, _tokens(15, cols, 4, seed=cols), top)
     _check_logprobs(x[:1], None, 0)
 
 
-@pytest.mark.parametrize('cols, period', [(131072, 256), (131072, 64), (131072, 2048), (32768, 1024), (262144, 8192)])
+@pytest.mark.parametrize('cols, period', [(131072, 256), (131072, 64), (131072, 2048), (32768, 1024), (262144, 8192),
+                                          (262144, 4096), (40000, 2048)])
 def test_alternatives_that_all_lie_in_few_lanes(cols, period):
     """The largest entries a fixed distance apart: where columns are dealt out to threads, a few threads hold them all."""
     x = _rows(2, cols, 'f32', seed=11)
@@ -138,8 +161,8 @@ def test_alternatives_that_all_lie_in_few_lanes(cols, period):
     x[0, at] = 50 + torch.arange(len(at), device='cuda').float() * 0.01
     x[1, at] = 50 - torch.arange(len(at), device='cuda').float() * 0.01
     for top in (3, 64):
-        _check_logprobs(x, None, top)
-    _check_logprobs(x.bfloat16(), None, 50)
+        _check_many(x, None, top, times=128)
+    _check_many(x.bfloat16(), None, 50, times=128)
 
 
 @pytest.mark.parametrize('cols', [40, 656, 5000, 20000])
@@ -149,7 +172,7 @@ def test_logprobs_of_ragged_rows(cols):
     for r, w in enumerate(widths.tolist()):
         x[r, max(0, min(w, cols)):] = math.nan
     x[9, :17] = -math.inf
-    _check_logprobs(x, _tokens(11, cols, 5), 20, widths)
+    _check_many(x, _tokens(11, cols, 5), 20, widths, times=25)
     _check_logprobs(x, _tokens(11, cols, 5), 0, widths.long())
 
 
@@ -165,6 +188,9 @@ def test_logprobs_of_strided_misaligned_and_expanded_rows(dtype):
     one = _rows(1, 3001, dtype)
     _check_logprobs(one.expand(5, 3001), _tokens(5, 3001, 2), 7)
     _check_logprobs(one.t()[:, :1].contiguous(), None, 1)
+    long = _rows(1, 600001, dtype)
+    want, many = _check_logprobs(long, None, 9), _scores().token_logprobs(long.expand(300, 600001), top=9)
+    assert torch.equal(many.top_index, want.top_index.expand(300, 9)) and (many.entropy - want.entropy).abs().max() < 1e-3
     _check_logprobs(_rows(50, 9, dtype)[:, 3:4], _tokens(50, 1, 1), 1)
 
 
