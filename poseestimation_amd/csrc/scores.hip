@@ -268,21 +268,14 @@ __device__ __forceinline__ void sc_join_wave(Stat& st) {
 // The same over a workgroup; every thread gets it.  The caller synchronises before wave_stat is used again.
 template <int WG>
 __device__ __forceinline__ void sc_join_block(Stat& st, Stat* wave_stat) {
+    constexpr int WAVES = WG / 64;
     sc_join_wave(st);
     if ((threadIdx.x & 63) == 0) wave_stat[threadIdx.x >> 6] = st;
     __syncthreads();
-    float m = wave_stat[0].m;
-#pragma unroll
-    for (int i = 1; i < WG / 64; ++i) m = fmaxf(m, wave_stat[i].m);
-    st = wave_stat[0];
-    sc_carry(st, m);
-#pragma unroll
-    for (int i = 1; i < WG / 64; ++i) {
-        Stat o = wave_stat[i];
-        sc_carry(o, m);
-        st.s += o.s;
-        st.w += o.w;
-    }
+    st = wave_stat[threadIdx.x & (WAVES - 1)];
+    sc_carry(st, sc_lanes(st.m, WAVES, FMaxOp()));
+    st.s = sc_lanes(st.s, WAVES, SumOp());
+    st.w = sc_lanes(st.w, WAVES, SumOp());
 }
 
 struct RowStat {
@@ -318,10 +311,25 @@ __device__ __forceinline__ int sc_width(const int32_t* widths, int64_t r, int co
     return widths ? pd_clampi(widths[r], 0, cols) : cols;
 }
 
-// Statistics and token log probabilities of row r, by threads i = 0 .. count - 1.
+// Thread i's token of row r (n_tok <= 64) and its score, asked for before the row is read.
+struct RowToken {
+    bool have, given;
+    float x;
+};
+
 template <typename X>
-__device__ __forceinline__ void sc_put_row(const LogprobArgs& a, int64_t r, const typename X::E* x, int n, const Stat& st,
-                                           const RowStat& q, int i, int count) {
+__device__ __forceinline__ RowToken sc_row_token(const LogprobArgs& a, int64_t r, const typename X::E* x, int n, int i) {
+    RowToken q = {i < a.n_tok, false, -INFINITY};
+    if (q.have) {
+        const int64_t tok = a.tokens[r * a.n_tok + i];
+        q.given = tok >= 0;
+        if (q.given && tok < n) q.x = X::get(x + tok);
+    }
+    return q;
+}
+
+// Statistics and token log probabilities of row r.
+__device__ __forceinline__ void sc_put_row(const LogprobArgs& a, int64_t r, const Stat& st, const RowStat& q, const RowToken& tok, int i) {
     if (i == 0) {
         if (a.stats) {
             a.stats[3 * r] = st.m;
@@ -330,12 +338,7 @@ __device__ __forceinline__ void sc_put_row(const LogprobArgs& a, int64_t r, cons
         }
         if (a.entropy) a.entropy[r] = q.entropy;
     }
-    for (int t = i; t < a.n_tok; t += count) {
-        const int64_t tok = a.tokens[r * a.n_tok + t];
-        float v = 0;
-        if (tok >= 0) v = q.empty ? -INFINITY : ((tok < n ? X::get(x + tok) : -INFINITY) - q.base) - q.log_sum;
-        a.logp[r * a.n_tok + t] = v;
-    }
+    if (tok.have) a.logp[r * a.n_tok + i] = !tok.given ? 0.0f : q.empty ? -INFINITY : (tok.x - q.base) - q.log_sum;
 }
 
 // Alternative k of row r; key 0: the row has no more scores, what lies behind it counts as -inf.
@@ -345,12 +348,29 @@ __device__ __forceinline__ void sc_put_top(const LogprobArgs& a, int64_t r, int 
     a.top_logp[at] = q.bad ? NAN : q.empty || !key ? -INFINITY : (sc_key_score(key) - q.base) - q.log_sum;
 }
 
-// The K-th largest of the orders o[0 .. N-1] of a wavefront's lanes, by its bits from the top; as soon as exactly K
-// values lie above the bits so far it is the least of them.
+// The K-th largest of the orders o[0 .. N-1] of a wavefront's lanes.  For a few, one maximum after the other; for more, by
+// its bits from the first in which they differ: as soon as exactly K values lie above the bits so far it is the least of
+// them.
 template <int N>
 __device__ __forceinline__ uint32_t sc_kth(const uint32_t* o, int K) {
-    uint32_t t = 0;
-    for (int bit = 31; bit >= 0; --bit) {
+    if (N == 1 && K <= 6) {
+        uint32_t left = o[0], top = sc_wave(left, MaxOp());
+        for (int k = 1; k < K; ++k) {
+            const uint64_t equal = __ballot(left == top);
+            if ((threadIdx.x & 63) == (uint32_t)__ffsll((unsigned long long)equal) - 1) left = 0;
+            top = sc_wave(left, MaxOp());
+        }
+        return top;
+    }
+    uint32_t hi = o[0], lo = o[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) hi = MaxOp()(hi, o[i]), lo = MinOp()(lo, o[i]);
+    hi = __builtin_amdgcn_readfirstlane(sc_wave(hi, MaxOp()));
+    lo = __builtin_amdgcn_readfirstlane(sc_wave(lo, MinOp()));
+    if (hi == lo) return hi;
+    const int bits = 32 - __clz(hi ^ lo);
+    uint32_t t = bits == 32 ? 0 : hi >> bits << bits;
+    for (int bit = bits - 1; bit >= 0; --bit) {
         const uint32_t trial = t | 1u << bit;
         int count = 0;
 #pragma unroll
@@ -384,6 +404,7 @@ __global__ __launch_bounds__(SC_WG) void k_token_logprobs_wave(LogprobArgs a) {
     for (int64_t r = (int64_t)blockIdx.x * SC_WAVES + wave; r < a.rows; r += (int64_t)gridDim.x * SC_WAVES) {
         const typename X::E* x = (const typename X::E*)a.x + r * a.stride;
         const int n = sc_width(a.widths, r, a.cols);
+        const RowToken tok = sc_row_token<X>(a, r, x, n, lane);
         float f[N];
 #pragma unroll
         for (int u = 0; u < NV; ++u) sc_read<X>(x, (u * 64 + lane) * V, n, f + u * V);
@@ -393,7 +414,7 @@ __global__ __launch_bounds__(SC_WG) void k_token_logprobs_wave(LogprobArgs a) {
         st.s = sc_wave(st.s, SumOp());
         st.w = sc_wave(st.w, SumOp());
         const RowStat q = sc_row_stat(st);
-        sc_put_row<X>(a, r, x, n, st, q, lane, 64);
+        sc_put_row(a, r, st, q, tok, lane);
         if (!a.top) continue;
         if (q.bad || q.empty) {
             if (lane < a.top) sc_put_top(a, r, lane, q.bad ? 0 : sc_key(-INFINITY, lane), q);
@@ -503,19 +524,22 @@ template <typename X, int WG, typename Put>
 __device__ void sc_top_block(TopShared<WG>& sh, const typename X::E* x, int begin, int end, int top, float lane_max, Put put) {
     constexpr int V = X::V;
     const int t = threadIdx.x;
-    // 256 parts of the columns, a thread's or four threads': the top-th largest of their maxima (top <= 64) is a bound
-    if constexpr (WG == 1024) {
-        lane_max = sc_lanes(lane_max, 4, FMaxOp());
-        if ((t & 3) == 0) sh.part_max[t / 4] = sc_order(lane_max);
-    } else {
-        sh.part_max[t] = sc_order(lane_max);
-    }
+    // The columns in 256 parts, or 64: the top-th largest of the parts' maxima is a bound.  Of 64 it is quicker found, and
+    // some top + top^2 / 128 scores reach it; at top = 64 it would be the least of them all.
+    const bool fine = top > 32;
+    lane_max = sc_lanes(lane_max, fine ? WG / 256 : WG / 64, FMaxOp());
+    if ((t & ((fine ? WG / 256 : WG / 64) - 1)) == 0) sh.part_max[t / (fine ? WG / 256 : WG / 64)] = sc_order(lane_max);
     __syncthreads();
     if (t < 64) {
-        uint32_t o[4];
+        uint32_t o[4], tau;
+        o[0] = sh.part_max[t];
+        if (fine) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = sh.part_max[t + 64 * i];
-        const uint32_t tau = sc_kth<4>(o, top);
+            for (int i = 1; i < 4; ++i) o[i] = sh.part_max[t + 64 * i];
+            tau = sc_kth<4>(o, top);
+        } else {
+            tau = sc_kth<1>(o, top);
+        }
         if (t == 0) sh.tau = tau;
     }
     __syncthreads();
@@ -609,6 +633,8 @@ __global__ __launch_bounds__(WG) void k_token_logprobs_block(LogprobArgs a) {
         const int n = sc_width(a.widths, r, a.cols);
         const int begin = slice * a.slice_cols < n ? slice * a.slice_cols : n;
         const int end = n - begin < a.slice_cols ? n : begin + a.slice_cols;
+        RowToken tok = {};
+        if (a.slices == 1) tok = sc_row_token<X>(a, r, x, n, t);
         Stat st = {-INFINITY, 0, 0};
         sc_u4 w[NV];
         if (AHEAD && begin + CHUNK <= end) sc_load_chunk<X, WG>(x + begin, t, w);
@@ -634,7 +660,7 @@ __global__ __launch_bounds__(WG) void k_token_logprobs_block(LogprobArgs a) {
         if (a.slices > 1) {
             if (t == 0) a.part[b] = st;
         } else {
-            sc_put_row<X>(a, r, x, n, st, q, t, WG);
+            sc_put_row(a, r, st, q, tok, t);
         }
         if constexpr (TOP) {
             if (a.slices > 1) {
@@ -665,6 +691,7 @@ __global__ __launch_bounds__(SC_WG) void k_token_logprobs_join(LogprobArgs a) {
     for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
         const typename X::E* x = (const typename X::E*)a.x + r * a.stride;
         const int n = sc_width(a.widths, r, a.cols);
+        const RowToken tok = sc_row_token<X>(a, r, x, n, t);
         Stat st = {-INFINITY, 0, 0};
         for (int i = t; i < a.slices; i += SC_WG) {
             Stat o = a.part[r * a.slices + i];
@@ -677,7 +704,7 @@ __global__ __launch_bounds__(SC_WG) void k_token_logprobs_join(LogprobArgs a) {
         if (t == 0) n_cand = 0;
         sc_join_block<SC_WG>(st, wave_stat);
         const RowStat q = sc_row_stat(st);
-        sc_put_row<X>(a, r, x, n, st, q, t, SC_WG);
+        sc_put_row(a, r, st, q, tok, t);
         if (a.top && (q.bad || q.empty)) {
             if (t < a.top) sc_put_top(a, r, t, q.bad ? 0 : sc_key(-INFINITY, t), q);
         } else if (a.top) {
@@ -1391,22 +1418,22 @@ static int sc_check_grad(const char* fn, const void* x, int dtype, int64_t rows,
     } while (0)
 
 // How a call with a workgroup to the row is cut: 256 threads a row where there are rows for every CU, 1024 with fewer; the
-// latter in slices of at least SC_SLICE_BYTES, as many as there are CUs for, which is what one CU reads in the time
-// that the join costs.
+// latter in slices of at least SC_SLICE_COLS, as many as there are CUs for.  A CU takes 9 us for that many, about what the
+// join of slices costs with its launch.
 #define SC_WAVE_COLS 2048
 #define SC_CUS 256
-#define SC_SLICE_BYTES (512 << 10)
+#define SC_SLICE_COLS (128 << 10)
 
 struct Cut {
     int wg, slices, slice_cols;
 };
 
-static Cut sc_cut(int dtype, int64_t rows, int64_t cols) {
+static Cut sc_cut(int64_t rows, int64_t cols) {
     Cut c;
     c.wg = rows >= SC_CUS ? SC_WG : 1024;
     const int64_t chunk = (int64_t)c.wg * SC_PER_THREAD, chunks = (cols + chunk - 1) / chunk;
     int64_t want = rows >= SC_CUS ? 1 : SC_CUS / rows;
-    const int64_t most = cols * sc_size(dtype) / SC_SLICE_BYTES, least = (chunks + SC_MAX_CHUNKS(c.wg) - 1) / SC_MAX_CHUNKS(c.wg);
+    const int64_t most = cols / SC_SLICE_COLS, least = (chunks + SC_MAX_CHUNKS(c.wg) - 1) / SC_MAX_CHUNKS(c.wg);
     if (want > most) want = most;
     if (want < least) want = least;
     const int64_t each = (chunks + want - 1) / want;
@@ -1419,7 +1446,7 @@ extern "C" uint64_t pd_token_logprobs_workspace(int dtype, int64_t rows, int64_t
     if (!sc_size(dtype) || rows < 1 || rows > INT32_MAX || columns <= SC_WAVE_COLS || columns > PD_MAX_COLUMNS || top < 0 ||
         top > PD_MAX_ALTERNATIVES)
         return 0;
-    const Cut c = sc_cut(dtype, rows, columns);
+    const Cut c = sc_cut(rows, columns);
     if (c.slices == 1) return 0;
     return (((uint64_t)rows * c.slices * sizeof(Stat) + 15) & ~15ull) + (uint64_t)rows * c.slices * top * sizeof(uint64_t);
 }
@@ -1475,7 +1502,7 @@ extern "C" int pd_token_logprobs(const void* logits, int dtype, int64_t rows, in
     }
     if (need && ((uintptr_t)workspace & 15)) return sc_fail(fn, "the workspace is not 16-byte aligned");
     LogprobArgs a = {logits, rows, row_stride, (int)columns, widths, tokens, n_tokens, top, logp, entropy, stats, top_logp, top_index};
-    const Cut cut = sc_cut(dtype, rows, columns);
+    const Cut cut = sc_cut(rows, columns);
     a.slices = cut.slices;
     a.slice_cols = cut.slice_cols;
     if (need) {

@@ -105,19 +105,25 @@ def token_logprobs(logits, tokens=None, top=0, widths=None):
     -inf, entropy 0, alternatives 0, 1, .. .  A row that holds a NaN or +inf: NaN, alternatives -1."""
     code, rows, columns, stride = _rows(logits, 'logits')
     dev = logits.device
-    n_tok, logp, top_logp, top_index, ws, ws_bytes = 0, None, None, None, None, 0
+    n_tok, shape, top = 0, None, int(top)
     if tokens is not None:
         tokens, shape = _tokens(tokens, rows, dev)
         n_tok = shape[1] if len(shape) == 2 else 1
-        logp = torch.empty(shape, dtype=torch.float32, device=dev)
     if widths is not None:
         widths = _like(widths, 'widths', torch.int32, ((rows,),), dev)
-    top = int(top)
-    if top > 0:
-        top_logp = torch.empty((rows, top), dtype=torch.float32, device=dev)
-        top_index = torch.empty((rows, top), dtype=torch.int32, device=dev)
-    entropy = torch.empty((rows,), dtype=torch.float32, device=dev)
-    stats = torch.empty((rows, 3), dtype=torch.float32, device=dev)
+    # one allocation for what a call returns, cut into the parts
+    k = max(top, 0)
+    store = torch.empty(rows * (n_tok + 2 * k + 4), dtype=torch.float32, device=dev)
+    entropy = store.as_strided((rows,), (1,))
+    stats = store.as_strided((rows, 3), (3, 1), rows)
+    logp = top_logp = top_index = ws = None
+    at = 4 * rows
+    if k:
+        top_logp = store.as_strided((rows, k), (k, 1), at)
+        top_index = store.view(torch.int32).as_strided((rows, k), (k, 1), at + rows * k)
+        at += 2 * rows * k
+    if shape is not None:
+        logp = store.as_strided(shape, (n_tok, 1) if len(shape) == 2 else (1,), at)
     ws_bytes = _ffi.lib().pd_token_logprobs_workspace(code, rows, columns, top)
     if ws_bytes:
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
