@@ -148,6 +148,13 @@ __device__ __forceinline__ void sc_pair(float v, float& p, float& q) {
     q = __uint_as_float(b);
 }
 template <int STEP>
+__device__ __forceinline__ void sc_pair(int v, int& p, int& q) {
+    uint32_t a, b;
+    sc_pair<STEP>((uint32_t)v, a, b);
+    p = (int)a;
+    q = (int)b;
+}
+template <int STEP>
 __device__ __forceinline__ void sc_pair(uint64_t v, uint64_t& p, uint64_t& q) {
     uint32_t a, b, c, d;
     sc_pair<STEP>((uint32_t)v, a, b);
@@ -254,6 +261,8 @@ __device__ __forceinline__ void sc_add(Stat& st, const float* x) {
         const float t = (x[i] - base) * SC_LOG2E, e = __builtin_amdgcn_exp2f(t);
         s[i & 1] += e;  // a NaN, or +inf, shows up here
         w[i & 1] = fmaf(e, sc_floor_t(t), w[i & 1]);
+        // (keeps W's sum here: left alone the compiler forms it behind S's, with every t and e in a register)
+        if (i % 8 == 7) asm volatile("" : "+v"(s[0]), "+v"(s[1]), "+v"(w[0]), "+v"(w[1]));
     }
     st.s += s[0] + s[1];
     st.w += w[0] + w[1];
@@ -302,7 +311,8 @@ struct LogprobArgs {
     int n_tok, top;
     float *logp, *entropy, *stats, *top_logp;
     int32_t* top_index;
-    int slices, slice_cols;  // a row in parts, one workgroup each (slice_cols a multiple of SC_CHUNK)
+    int lanes;               // to a short row
+    int slices, slice_cols;  // a long row in parts, one workgroup each (slice_cols a multiple of its chunk)
     Stat* part;              // [rows][slices]
     uint64_t* part_keys;     // [rows][slices][top], 0: none
 };
@@ -387,76 +397,128 @@ __device__ __forceinline__ uint32_t sc_kth(const uint32_t* o, int K) {
     return t;
 }
 
-// ---- a wavefront to the row: up to 2048 columns, all of them in registers ---------------------
+// ---- 16, 32 or 64 lanes to the row: up to 2048 columns, all of them in registers ----------------
 //
-// Bound by instruction issue, not by memory: a row of a few hundred columns is some ten instructions a score and
-// as many again a row for the reductions and the alternatives, so nothing is exchanged through LDS but the handful
-// of candidates, and wavefronts do not wait for each other.
+// Bound by instruction issue and latency, not by memory: some ten instructions a score, and a few hundred for the
+// reductions, the alternatives and the results, which the rows of a wavefront share.  So rows are packed as tightly as
+// their number allows; nothing is exchanged through LDS but the handful of candidates, and wavefronts do not wait for
+// each other.
 
-#define SC_WAVE_CAND 128  // candidates of a row; more (equal scores) are found one by one
+#define SC_WAVE_CAND 128  // candidates of a wavefront's rows
 
 template <typename X, int NV>
-__global__ __launch_bounds__(SC_WG) void k_token_logprobs_wave(LogprobArgs a) {
+__global__ __launch_bounds__(SC_WG) void k_token_logprobs_rows(LogprobArgs a) {
     constexpr int V = X::V, N = NV * V;
     __shared__ uint64_t cand[SC_WAVES][SC_WAVE_CAND];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    uint64_t* mine = cand[wave];
-    for (int64_t r = (int64_t)blockIdx.x * SC_WAVES + wave; r < a.rows; r += (int64_t)gridDim.x * SC_WAVES) {
-        const typename X::E* x = (const typename X::E*)a.x + r * a.stride;
-        const int n = sc_width(a.widths, r, a.cols);
-        const RowToken tok = sc_row_token<X>(a, r, x, n, lane);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int L = a.lanes, l = lane & (L - 1), first = lane & ~(L - 1), per_wave = 64 / L;
+    const uint64_t row_lanes = (L == 64 ? ~0ull : (1ull << L) - 1) << first, before = row_lanes & ((1ull << lane) - 1);
+    const int room = SC_WAVE_CAND / per_wave;
+    uint64_t* mine = cand[wave] + first / L * room;
+    const int64_t tiles = (a.rows + per_wave - 1) / per_wave;
+    for (int64_t tile = (int64_t)blockIdx.x * SC_WAVES + wave; tile < tiles; tile += (int64_t)gridDim.x * SC_WAVES) {
+        const int64_t r = tile * per_wave + lane / L;
+        const bool on = r < a.rows;
+        const typename X::E* x = (const typename X::E*)a.x + (on ? r : a.rows - 1) * a.stride;
+        const int n = on ? sc_width(a.widths, r, a.cols) : 0;
+        RowToken tok = {};
+        if (on && a.n_tok <= L) tok = sc_row_token<X>(a, r, x, n, l);
         float f[N];
 #pragma unroll
-        for (int u = 0; u < NV; ++u) sc_read<X>(x, (u * 64 + lane) * V, n, f + u * V);
+        for (int u = 0; u < NV; ++u) sc_read<X>(x, (u * L + l) * V, n, f + u * V);
         const float m = sc_max<N>(f, -INFINITY);
-        Stat st = {sc_wave(m, FMaxOp()), 0, 0};
+        Stat st = {sc_lanes(m, L, FMaxOp()), 0, 0};
         sc_add<N>(st, f);
-        st.s = sc_wave(st.s, SumOp());
-        st.w = sc_wave(st.w, SumOp());
+        st.s = sc_lanes(st.s, L, SumOp());
+        st.w = sc_lanes(st.w, L, SumOp());
         const RowStat q = sc_row_stat(st);
-        sc_put_row(a, r, st, q, tok, lane);
-        if (!a.top) continue;
-        if (q.bad || q.empty) {
-            if (lane < a.top) sc_put_top(a, r, lane, q.bad ? 0 : sc_key(-INFINITY, lane), q);
-            continue;
+        if (on) {
+            sc_put_row(a, r, st, q, tok, l);
+            if (a.n_tok > L)
+                for (int i = l; i < a.n_tok; i += L) sc_put_row(a, r, st, q, sc_row_token<X>(a, r, x, n, i), i);
         }
-        const uint32_t mo = sc_order(m);
-        const float tau = sc_unorder(sc_kth<1>(&mo, a.top));
-        int count = 0;
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int at = ((i / V) * 64 + lane) * V + i % V;
-            const bool in = f[i] >= tau && at < n;
-            const uint64_t mask = __ballot(in);
-            if (mask) {
-                const int to = count + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
-                if (in && to < SC_WAVE_CAND) mine[to] = sc_key(f[i], at);
-                count += __popcll(mask);
+        if (!a.top) continue;
+        const bool plain = on && !q.bad && !q.empty;
+        float tau;
+        if (L == 64 && a.top > 6) {
+            const uint32_t o = sc_order(m);
+            tau = sc_unorder(sc_kth<1>(&o, a.top));
+        } else {  // a few: one maximum after the other
+            float left = m;
+            tau = sc_lanes(left, L, FMaxOp());
+            for (int k = 1; k < a.top; ++k) {
+                const uint64_t equal = __ballot(left == tau) & row_lanes;
+                if (lane == __ffsll((unsigned long long)equal) - 1) left = -INFINITY;
+                tau = sc_lanes(left, L, FMaxOp());
             }
         }
+        // What reaches tau is marked without a branch, and the few are read again: N branches with a key each would take
+        // 80 registers more.
+        uint32_t take = 0;
+#pragma unroll
+        for (int i = N - 1; i >= 0; --i) take = take + take + (f[i] >= tau);
+        if (__any(tau == -INFINITY)) {  // then what lies behind the row does, too
+            uint32_t valid = 0;
+            for (int u = 0; u < NV; ++u) valid |= ((1u << pd_clampi(n - (u * L + l) * V, 0, V)) - 1) << (u * V);
+            take &= valid;
+        }
+        if (!plain) take = 0;
+        int count = sc_lanes(__popc(take), L, SumOp());
+        if (__any(count > room)) {
+            // Too many scores equal to tau (a masked row, a constant one): of those the first that make up the number.
+            uint32_t above = 0;
+#pragma unroll
+            for (int i = N - 1; i >= 0; --i) above = above + above + (f[i] > tau);
+            if (!plain) above = 0;
+            const uint32_t equal = take & ~above;
+            const bool cut = count > room;
+            int have = sc_lanes(__popc(above), L, SumOp());
+            if (cut) take = above;
+            for (int u = 0; u < NV; ++u) {
+                uint32_t bits = equal >> (u * V) & ((1u << V) - 1);
+                const int c = __popc(bits);
+                int upto = c;  // an inclusive scan over the row's lanes
+                for (int d = 1; d < L; d <<= 1) {
+                    const int o = __shfl_up(upto, d, L);
+                    if (l >= d) upto += o;
+                }
+                for (int drop = c - pd_clampi(a.top - have - (upto - c), 0, c); drop > 0; --drop) bits &= ~(1u << (31 - __clz((int)bits)));
+                if (cut) take |= bits << (u * V);
+                have += __shfl(upto, first + L - 1);
+            }
+            count = sc_lanes(__popc(take), L, SumOp());
+        }
+        const bool fits = !__any(count > room);
+        int from = 0;
+        while (fits && __any(take != 0)) {
+            const int i = __ffs((int)take) - 1, at = i / V * L * V + (i & (V - 1)) + l * V;
+            const bool in = take != 0;
+            take &= take - 1;
+            const uint64_t mask = __ballot(in);
+            if (in) mine[from + __popcll(mask & before)] = sc_key(X::get(x + at), at);
+            from += __popcll(mask & row_lanes);
+        }
         pd_wave_sync();
-        if (count <= SC_WAVE_CAND) {
-            for (int i = lane; i < count; i += 64) {
+        if (fits) {
+            for (int i = l; i < count; i += L) {
                 const uint64_t key = mine[i];
                 const int rank = sc_rank(mine, count, key);
                 if (rank < a.top) sc_put_top(a, r, rank, key, q);
             }
-            if (lane >= count && lane < a.top) sc_put_top(a, r, lane, 0, q);
+            if (on && l < a.top && (!plain || l >= count)) sc_put_top(a, r, l, q.empty ? sc_key(-INFINITY, l) : 0, q);
         } else {
-            uint64_t prev = ~0ull;
+            uint64_t prev = ~0ull;  // many large scores in few lanes: one after the other
             for (int k = 0; k < a.top; ++k) {
                 uint64_t best = 0;
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    const int at = ((i / V) * 64 + lane) * V + i % V;
-                    const uint64_t key = sc_key(f[i], at);
-                    if (at < n && key < prev && key > best) best = key;
+                for (int at = l; at < n; at += L) {
+                    const uint64_t key = sc_key(X::get(x + at), at);
+                    if (key < prev && key > best) best = key;
                 }
-                prev = sc_wave(best, MaxOp());
-                if (lane == 0) sc_put_top(a, r, k, prev, q);
+                prev = sc_lanes(best, L, MaxOp());
+                if (on && l == 0) sc_put_top(a, r, k, prev, q);
             }
         }
-        pd_wave_sync();  // the next row's candidates go to the same place
+        pd_wave_sync();  // the next rows' candidates go to the same place
     }
 }
 
@@ -622,7 +684,8 @@ struct Nothing {};
 template <typename X, int WG, bool TOP>
 __global__ __launch_bounds__(WG) void k_token_logprobs_block(LogprobArgs a) {
     constexpr int V = X::V, NV = SC_PER_THREAD / V, CHUNK = WG * SC_PER_THREAD, WAVES = WG / 64;
-    constexpr bool AHEAD = WG == 1024;  // few workgroups: nobody else to fill the time between a load and its use
+    // few workgroups: nobody else to fill the time between a load and its use (float32: no registers for it)
+    constexpr bool AHEAD = WG == 1024 && V == 8;
     __shared__ Stat wave_stat[WAVES];
     __shared__ typename std::conditional<TOP, TopShared<WG>, Nothing>::type sh;
     const int t = threadIdx.x;
@@ -1417,6 +1480,17 @@ static int sc_check_grad(const char* fn, const void* x, int dtype, int64_t rows,
             hipLaunchKernelGGL((kernel<F16>), dim3(grid), dim3(SC_WG), 0, (hipStream_t)(stream), args);   \
     } while (0)
 
+// Lanes to a row of up to SC_WAVE_COLS columns: the fewest with at most 32 scores to a lane, as long as that leaves
+// SC_ROW_WAVES wavefronts, four to a SIMD, and as the lanes' maxima bound the alternatives well.
+#define SC_ROW_WAVES 4096
+
+static int sc_row_lanes(int64_t rows, int64_t cols, int top) {
+    int lanes = 64;
+    const int least = top <= 8 ? 16 : top <= 16 ? 32 : 64;
+    while (lanes > least && cols <= lanes / 2 * 32 && rows * (lanes / 2) >= 64 * SC_ROW_WAVES) lanes /= 2;
+    return lanes;
+}
+
 // How a call with a workgroup to the row is cut: 256 threads a row where there are rows for every CU, 1024 with fewer; the
 // latter in slices of at least SC_SLICE_COLS, as many as there are CUs for.  A CU takes 9 us for that many, about what the
 // join of slices costs with its launch.
@@ -1463,18 +1537,21 @@ static void sc_launch_logprobs_block(const LogprobArgs& a, hipStream_t stream) {
 
 template <typename X>
 static void sc_launch_logprobs(const LogprobArgs& a, int wg_size, hipStream_t stream) {
-    const dim3 wg(SC_WG);
     if (a.cols <= SC_WAVE_COLS) {
-        const dim3 grid(sc_grid((a.rows + SC_WAVES - 1) / SC_WAVES));
-        const int vecs = (a.cols + 64 * X::V - 1) / (64 * X::V);
+        const dim3 grid(sc_grid((a.rows * a.lanes + SC_WG - 1) / SC_WG)), wg(SC_WG);
+        const int vecs = (a.cols + a.lanes * X::V - 1) / (a.lanes * X::V);
         if (vecs <= 1)
-            hipLaunchKernelGGL((k_token_logprobs_wave<X, 1>), grid, wg, 0, stream, a);
+            hipLaunchKernelGGL((k_token_logprobs_rows<X, 1>), grid, wg, 0, stream, a);
         else if (vecs <= 2)
-            hipLaunchKernelGGL((k_token_logprobs_wave<X, 2>), grid, wg, 0, stream, a);
+            hipLaunchKernelGGL((k_token_logprobs_rows<X, 2>), grid, wg, 0, stream, a);
+        else if (vecs <= 3)
+            hipLaunchKernelGGL((k_token_logprobs_rows<X, 3>), grid, wg, 0, stream, a);
         else if (vecs <= 4)
-            hipLaunchKernelGGL((k_token_logprobs_wave<X, 4>), grid, wg, 0, stream, a);
+            hipLaunchKernelGGL((k_token_logprobs_rows<X, 4>), grid, wg, 0, stream, a);
+        else if (vecs <= 6)
+            hipLaunchKernelGGL((k_token_logprobs_rows<X, 24 / X::V>), grid, wg, 0, stream, a);
         else
-            hipLaunchKernelGGL((k_token_logprobs_wave<X, SC_WAVE_COLS / 64 / X::V>), grid, wg, 0, stream, a);
+            hipLaunchKernelGGL((k_token_logprobs_rows<X, 32 / X::V>), grid, wg, 0, stream, a);
         return;
     }
     if (wg_size == SC_WG)
@@ -1503,6 +1580,7 @@ extern "C" int pd_token_logprobs(const void* logits, int dtype, int64_t rows, in
     if (need && ((uintptr_t)workspace & 15)) return sc_fail(fn, "the workspace is not 16-byte aligned");
     LogprobArgs a = {logits, rows, row_stride, (int)columns, widths, tokens, n_tokens, top, logp, entropy, stats, top_logp, top_index};
     const Cut cut = sc_cut(rows, columns);
+    a.lanes = sc_row_lanes(rows, columns, top);
     a.slices = cut.slices;
     a.slice_cols = cut.slice_cols;
     if (need) {
