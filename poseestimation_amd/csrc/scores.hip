@@ -524,11 +524,11 @@ __global__ __launch_bounds__(SC_WG) void k_token_logprobs_rows(LogprobArgs a) {
 
 // ---- a workgroup to the row, or to a slice of it ------------------------------------------------
 //
-// Chunks of WG * 32 columns, 32 to a thread in 16-byte loads.  With many rows: 256 threads, six to eight workgroups
-// to a CU keep the loads coming while others reduce; bound by the memory (4096 x 131072 bfloat16 with five alternatives:
-// 199 us, 5.4 TB/s).  With fewer rows than CUs: 1024 threads that load a chunk while they add the one before; bound by
-// what one CU can have in flight, and by the latency of the steps behind the last load.  Rows that would take one CU long
-// are cut into slices, joined by k_token_logprobs_join.
+// Chunks of WG * 32 columns, 32 to a thread in 16-byte loads.  With many rows: 64 or 256 threads, and workgroups enough on
+// a CU to keep the loads coming while others reduce; bound by the memory (4096 x 131072 bfloat16 with five alternatives:
+// 196 us, 5.5 TB/s).  With few long rows: 1024 threads that load a chunk while they add the one before; bound by
+// instruction issue on the one CU (131072 columns 9 us) and by the latency of the steps behind the last load.  Rows that would
+// take one CU longer are cut into slices, joined by k_token_logprobs_join.
 
 #define SC_PER_THREAD 32
 #define SC_MAX_CHUNKS(WG) ((WG) == 1024 ? 8 : 16)
@@ -588,9 +588,11 @@ __device__ void sc_top_block(TopShared<WG>& sh, const typename X::E* x, int begi
     const int t = threadIdx.x;
     // The columns in 256 parts, or 64: the top-th largest of the parts' maxima is a bound.  Of 64 it is quicker found, and
     // some top + top^2 / 128 scores reach it; at top = 64 it would be the least of them all.
-    const bool fine = top > 32;
-    lane_max = sc_lanes(lane_max, fine ? WG / 256 : WG / 64, FMaxOp());
-    if ((t & ((fine ? WG / 256 : WG / 64) - 1)) == 0) sh.part_max[t / (fine ? WG / 256 : WG / 64)] = sc_order(lane_max);
+    // (A workgroup of 64 has 64, and is not given more than 32 alternatives to find.)
+    const bool fine = WG > 64 && top > 32;
+    const int part = fine ? WG / 256 : WG / 64;  // threads to a part
+    lane_max = sc_lanes(lane_max, part, FMaxOp());
+    if ((t & (part - 1)) == 0) sh.part_max[t / part] = sc_order(lane_max);
     __syncthreads();
     if (t < 64) {
         uint32_t o[4], tau;
@@ -1491,9 +1493,12 @@ static int sc_row_lanes(int64_t rows, int64_t cols, int top) {
     return lanes;
 }
 
-// How a call with a workgroup to the row is cut: 256 threads a row where there are rows for every CU, 1024 with fewer; the
-// latter in slices of at least SC_SLICE_COLS, as many as there are CUs for.  A CU takes 9 us for that many, about what the
-// join of slices costs with its launch.
+// How a call with a workgroup to the row is cut.  Measured in the kernel, five alternatives, bfloat16, 64 / 256 / 1024
+// threads: 8192 x 4096 22 / 43 / 224 us, 16 x 4096 6.1 / 6.2 / 8.1, 4096 x 16384 28 / 31 / 117, 1400 x 16384 17 / 15 / 45,
+// 200 x 16384 10.7 / 6.8 / 8.6, 4096 x 131072 233 / 214 / 261, 255 x 131072 25 / 24 / 19.  So: one wavefront for rows of up to
+// 4096 columns, and up to 32768 where there are eight for every CU (it waits for no other at a row's end); 1024 threads for
+// long rows that leave CUs idle, in slices of at least SC_SLICE_COLS, as many as there are CUs for (a CU takes 9 us for that
+// many, about what the join of slices costs with its launch); 256 otherwise.  More than 32 alternatives need 256 parts.
 #define SC_WAVE_COLS 2048
 #define SC_CUS 256
 #define SC_SLICE_COLS (128 << 10)
@@ -1502,11 +1507,14 @@ struct Cut {
     int wg, slices, slice_cols;
 };
 
-static Cut sc_cut(int64_t rows, int64_t cols) {
+static Cut sc_cut(int64_t rows, int64_t cols, int top) {
     Cut c;
-    c.wg = rows >= SC_CUS ? SC_WG : 1024;
+    if (top <= 32 && (cols <= 4096 || (cols <= 32768 && rows >= 8 * SC_CUS)))
+        c.wg = 64;
+    else
+        c.wg = rows < SC_CUS && cols > 32768 ? 1024 : SC_WG;
     const int64_t chunk = (int64_t)c.wg * SC_PER_THREAD, chunks = (cols + chunk - 1) / chunk;
-    int64_t want = rows >= SC_CUS ? 1 : SC_CUS / rows;
+    int64_t want = c.wg < 1024 ? 1 : SC_CUS / rows;
     const int64_t most = cols / SC_SLICE_COLS, least = (chunks + SC_MAX_CHUNKS(c.wg) - 1) / SC_MAX_CHUNKS(c.wg);
     if (want > most) want = most;
     if (want < least) want = least;
@@ -1520,7 +1528,7 @@ extern "C" uint64_t pd_token_logprobs_workspace(int dtype, int64_t rows, int64_t
     if (!sc_size(dtype) || rows < 1 || rows > INT32_MAX || columns <= SC_WAVE_COLS || columns > PD_MAX_COLUMNS || top < 0 ||
         top > PD_MAX_ALTERNATIVES)
         return 0;
-    const Cut c = sc_cut(rows, columns);
+    const Cut c = sc_cut(rows, columns, top);
     if (c.slices == 1) return 0;
     return (((uint64_t)rows * c.slices * sizeof(Stat) + 15) & ~15ull) + (uint64_t)rows * c.slices * top * sizeof(uint64_t);
 }
@@ -1554,7 +1562,9 @@ static void sc_launch_logprobs(const LogprobArgs& a, int wg_size, hipStream_t st
             hipLaunchKernelGGL((k_token_logprobs_rows<X, 32 / X::V>), grid, wg, 0, stream, a);
         return;
     }
-    if (wg_size == SC_WG)
+    if (wg_size == 64)
+        sc_launch_logprobs_block<X, 64>(a, stream);
+    else if (wg_size == SC_WG)
         sc_launch_logprobs_block<X, SC_WG>(a, stream);
     else
         sc_launch_logprobs_block<X, 1024>(a, stream);
@@ -1579,7 +1589,7 @@ extern "C" int pd_token_logprobs(const void* logits, int dtype, int64_t rows, in
     }
     if (need && ((uintptr_t)workspace & 15)) return sc_fail(fn, "the workspace is not 16-byte aligned");
     LogprobArgs a = {logits, rows, row_stride, (int)columns, widths, tokens, n_tokens, top, logp, entropy, stats, top_logp, top_index};
-    const Cut cut = sc_cut(rows, columns);
+    const Cut cut = sc_cut(rows, columns, top);
     a.lanes = sc_row_lanes(rows, columns, top);
     a.slices = cut.slices;
     a.slice_cols = cut.slice_cols;

@@ -46,8 +46,8 @@ BAD = [
     (_logprobs, dict(n=-1), 'n_tokens'), (_logprobs, dict(n=65), 'n_tokens'), (_logprobs, dict(tokens=None), 'tokens'),
     (_logprobs, dict(logp=None), 'tokens'), (_logprobs, dict(top=-1), 'top'), (_logprobs, dict(top=65), 'top'),
     (_logprobs, dict(cols=5, top=6), 'top'), (_logprobs, dict(tl=None), 'top_logp'), (_logprobs, dict(ti=None), 'top_logp'),
-    (_logprobs, dict(cols=200000), 'workspace'), (_logprobs, dict(cols=200000, ws=P, ws_bytes=16), 'workspace'),
-    (_logprobs, dict(cols=200000, ws=P + 8, ws_bytes=1 << 20), 'aligned'),
+    (_logprobs, dict(cols=1 << 20, stride=1 << 20), 'workspace'), (_logprobs, dict(cols=1 << 20, ws=P, ws_bytes=16), 'workspace'),
+    (_logprobs, dict(cols=1 << 20, ws=P + 8, ws_bytes=1 << 20), 'aligned'),
     (_logprobs_grad, dict(dtype=_ffi.U8), 'PD_F32'), (_logprobs_grad, dict(cols=0), 'columns'),
     (_logprobs_grad, dict(stats=None), 'stats'), (_logprobs_grad, dict(out=None), 'grad'),
     (_logprobs_grad, dict(out=2 * P + 1), 'aligned'), (_logprobs_grad, dict(out_stride=99), 'overlap'),
