@@ -1021,15 +1021,18 @@ __device__ __forceinline__ void sc_route_row(const RouteArgs& a, int64_t r, int 
     double m = 0, total = 0;
     if (!a.sigmoid) {
         float big = -INFINITY;
+#pragma nounroll
         for (int j = lane; j < E; j += 64) big = fmaxf(big, sc_logit(a.x, a.dtype, row + j));
         big = sc_wave(big, FMaxOp());
         if (big > -INFINITY) {
             m = big;
+#pragma nounroll
             for (int j = lane; j < E; j += 64) total += exp(sc_logit(a.x, a.dtype, row + j) - m);
         }
         total = sc_wave(total, SumOp());
     }
     const bool by_p = a.bias || (a.groups > 1 && a.top2);  // else by the logits alone
+#pragma nounroll
     for (int j = lane; j < E; j += 64) {
         const double x = sc_logit(a.x, a.dtype, row + j);
         double v = x;
@@ -1043,6 +1046,7 @@ __device__ __forceinline__ void sc_route_row(const RouteArgs& a, int64_t r, int 
         double mine = -INFINITY;  // lane g: group g's
         if (lane < a.groups) {
             double b1 = -INFINITY, b2 = -INFINITY;
+#pragma nounroll
             for (int j = lane * a.per_group; j < (lane + 1) * a.per_group; ++j) {
                 b2 = fmax(b2, fmin(b1, by[j]));
                 b1 = fmax(b1, by[j]);
@@ -1050,20 +1054,24 @@ __device__ __forceinline__ void sc_route_row(const RouteArgs& a, int64_t r, int 
             mine = a.top2 && a.per_group > 1 ? b1 + b2 : b1;
         }
         int rank = 0;
+#pragma nounroll
         for (int g = 0; g < a.groups; ++g) {
             const double o = __shfl(mine, g);
             rank += o > mine || (o == mine && g < lane);
         }
         kept = __ballot(lane < a.groups && rank < a.top_groups);
     }
+#pragma nounroll
     for (int j = lane; j < E; j += 64) {
         if (by_p && !a.bias) by[j] = fmax((double)sc_logit(a.x, a.dtype, row + j), -1e300);  // p counted for the groups only
         if (!(kept >> (j / a.per_group) & 1)) by[j] = -INFINITY;
     }
     int chosen = -1;
+#pragma nounroll
     for (int k = 0; k < a.top; ++k) {
         double best = -INFINITY;
         int at = E;
+#pragma nounroll
         for (int j = lane; j < E; j += 64)
             if (by[j] > best) best = by[j], at = j;
         const double top = sc_wave(best, MaxOp());
@@ -1198,11 +1206,6 @@ __global__ __launch_bounds__(SC_WG) void k_route(RouteArgs a) {
     const int have = g < a.groups ? pd_clampi(a.per_group - in_group, 0, EPL) : 0;
     const bool full = __ballot(have == EPL) == ~0ull;
     const bool biased = CLOSE && a.bias;
-    float bias[CLOSE ? EPL : 1];
-    if constexpr (CLOSE) {
-#pragma unroll
-        for (int j = 0; j < EPL; ++j) bias[j] = biased && j < have ? a.bias[place + j] : 0.0f;
-    }
     const int64_t tiles = (a.rows + per_wave - 1) / per_wave;
     for (int64_t tile = (int64_t)blockIdx.x * SC_WAVES + wave; tile < tiles; tile += (int64_t)gridDim.x * SC_WAVES) {
         const int64_t r = tile * per_wave + lane / L, row = r < a.rows ? r : a.rows - 1;
@@ -1248,8 +1251,12 @@ __global__ __launch_bounds__(SC_WG) void k_route(RouteArgs a) {
                 // exponents' |t| 2^t, the exponential, the division; the difference of two by twice that
                 tol = 0x1p-17f * inv;
             }
+            if (biased) {  // (from the L1: the same for every row)
+                float b[EPL];
+                sc_route_read<F32, EPL>(a.bias, place, have, full, b);
 #pragma unroll
-            for (int j = 0; j < EPL; ++j) s[j] += bias[j];
+                for (int j = 0; j < EPL; ++j) s[j] += b[j];
+            }
         }
         if (a.groups > 1) {
             float b1 = -INFINITY, b2 = -INFINITY;
@@ -1337,26 +1344,28 @@ __global__ __launch_bounds__(SC_WG) void k_route(RouteArgs a) {
                     if (k + 1 < a.top && !(best[k] - best[k + 1] > tol + 0x1p-22 * fabs(best[k]))) close |= 1u << k;
                     last = k + 1 == a.top - 1 ? best[k + 1] : last;
                 }
-                if (on && !bad && close) {
-#pragma unroll
-                    for (int k = 0; k + 1 < KP; ++k)
-                        if (close >> k & 1) {
-                            const int p0 = Key::place(best[k]), p1 = Key::place(best[k + 1]);
-                            again |= sc_logit(a.x, a.dtype, row * a.stride + p0) != sc_logit(a.x, a.dtype, row * a.stride + p1) ||
-                                     a.bias[p0] != a.bias[p1];
-                        }
+                if (!on || bad) close = 0;
+                while (__any(close != 0)) {  // lane k of the row holds the k-th place
+                    const int k = close ? __ffs((int)close) - 1 : 0, p0 = __shfl(idx, first + k), p1 = __shfl(idx, first + k + 1);
+                    if (close)
+                        again |= sc_logit(a.x, a.dtype, row * a.stride + p0) != sc_logit(a.x, a.dtype, row * a.stride + p1) ||
+                                 a.bias[p0] != a.bias[p1];
+                    close &= close - 1;
                 }
                 // An expert too close to the last one chosen, on either side: the choice stands if they are equal.
                 const float edge = (float)last, off = tol + 0x1p-22f * fabsf(edge);
                 const int pl = Key::place(last);
-                bool near = false;
+                uint32_t near = 0;
 #pragma unroll
-                for (int j = 0; j < EPL; ++j) near |= !(fabsf(s[j] - edge) > off) && place + j != pl;
+                for (int j = EPL - 1; j >= 0; --j) near = near + near + !(fabsf(s[j] - edge) > off);
+                if (pl >= place && pl < place + EPL) near &= ~(1u << (pl - place));
                 if (on && !bad && near && kept) {
                     const float xl = sc_logit(a.x, a.dtype, row * a.stride + pl), bl = a.bias[pl];
-#pragma unroll
-                    for (int j = 0; j < EPL; ++j)
-                        again |= j < have && !(fabsf(s[j] - edge) > off) && place + j != pl && (x[j] != xl || bias[j] != bl);
+                    for (; near; near &= near - 1) {
+                        const int j = __ffs((int)near) - 1;
+                        if (j < have)
+                            again |= sc_logit(a.x, a.dtype, row * a.stride + place + j) != xl || a.bias[place + j] != bl;
+                    }
                 }
             }
             uint64_t todo = __ballot(again && on && !bad);
@@ -1381,48 +1390,78 @@ struct RouteGradArgs {
     const float* g;
     void* out;
     int64_t out_stride;
+    int lanes;
 };
 
-template <typename X>
+// With w the chosen experts' p, divided by their sum where they are renormalised:
+//   renormalised, or sigmoid:  dx_i = w_i (g_i - sum g w) [renormalised, else w_i g_i], times 1 - p_i for a sigmoid, at the
+//                              chosen; 0 elsewhere, and the other logits are not read;
+//   softmax as it is:          dx_j = p_j ([j chosen] g_j - sum over the chosen of g_i p_i), which reaches every expert.
+// A row's lanes put the chosen experts' values into the row's zeroes in LDS (an expert named twice adds up) and write it out
+// in 16-byte pieces.  Bound by the memory and the latency of index -> logit.
+template <typename X, int NV, bool DENSE>
 __global__ __launch_bounds__(SC_WG) void k_route_grad(RouteGradArgs a) {
-    const int lane = threadIdx.x & 63;
-    for (int64_t r = (int64_t)blockIdx.x * (SC_WG / 64) + (threadIdx.x >> 6); r < a.rows; r += (int64_t)gridDim.x * (SC_WG / 64)) {
-        const typename X::E* x = (const typename X::E*)a.x + r * a.stride;
-        typename X::E* out = (typename X::E*)a.out + r * a.out_stride;
-        const int E = a.experts;
-        const int idx = lane < a.top ? a.index[r * a.top + lane] : -1;
+    constexpr int V = X::V;
+    __shared__ __align__(16) float rows_acc[SC_WAVES][PD_MAX_EXPERTS];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int L = a.lanes, l = lane & (L - 1), per_wave = 64 / L, E = a.experts;
+    const int padded = (E + 7) & ~7;  // 64 / L rows of at most 16 L
+    float* acc = rows_acc[wave] + lane / L * padded;
+    const int64_t tiles = (a.rows + per_wave - 1) / per_wave;
+    for (int64_t tile = (int64_t)blockIdx.x * SC_WAVES + wave; tile < tiles; tile += (int64_t)gridDim.x * SC_WAVES) {
+        const int64_t r = tile * per_wave + lane / L;
+        const bool on = r < a.rows;
+        const typename X::E* x = (const typename X::E*)a.x + (on ? r : 0) * a.stride;
+        const int idx = on && l < a.top ? a.index[r * a.top + l] : -1;
         const bool have = idx >= 0 && idx < E;
-        const float g = have ? a.g[r * a.top + lane] * a.scale : 0.0f;
+        const float g = have ? a.g[r * a.top + l] * a.scale : 0.0f;
         const float xi = have ? X::get(x + idx) : -INFINITY;
-        const bool dense = !a.sigmoid && !a.renorm;
-        float m = 0, total = 0, wgt, c;
-        if (a.sigmoid || a.renorm) {
-            wgt = sc_chosen_share(xi, have, a.sigmoid, a.renorm, 64);
-            const float sum = a.renorm ? sc_wave(wgt * g, SumOp()) : 0.0f;
-            c = wgt * (g - sum);
-            if (a.sigmoid) c *= xi > 0 ? expf(-xi) / (1 + expf(-xi)) : 1 / (1 + expf(xi));  // 1 - p
-        } else {
-            m = -INFINITY;
-            for (int j = lane; j < E; j += 64) m = fmaxf(m, X::get(x + j));
-            m = sc_wave(m, MaxOp());
-            if (m > -INFINITY)
-                for (int j = lane; j < E; j += 64) total += expf(X::get(x + j) - m);
-            total = sc_wave(total, SumOp());
-            wgt = have && total != 0 ? expf(xi - m) / total : 0.0f;
-            c = wgt * g;
-        }
-        const float all = dense ? sc_wave(c, SumOp()) : 0.0f;
-        for (int j0 = 0; j0 < E; j0 += 64) {
-            const int j = j0 + lane;
-            float d = 0;
-            if (dense && j < E && total != 0) d = -(expf(X::get(x + j) - m) / total) * all;
-            for (int k = 0; k < a.top; ++k) {
-                const int at = __shfl(have ? idx : -1, k);
-                const float v = __shfl(c, k);
-                if (at == j) d += v;
+        for (int j = 4 * l; j < padded; j += 4 * L) *(float4*)(acc + j) = make_float4(0, 0, 0, 0);
+        float f[DENSE ? NV * V : 1], m = 0, inv = 0, c, all = 0;
+        if constexpr (DENSE) {
+#pragma unroll
+            for (int v = 0; v < NV; ++v) sc_read<X>(x, (v * L + l) * V, on ? E : 0, f + v * V);
+            m = sc_lanes(sc_max<NV * V>(f, -INFINITY), L, FMaxOp());
+            m = m == -INFINITY ? 0.0f : m;
+            float total = 0;
+#pragma unroll
+            for (int i = 0; i < NV * V; ++i) {
+                f[i] = __builtin_amdgcn_exp2f((f[i] - m) * SC_LOG2E);
+                total += f[i];
             }
-            if (j < E) X::put(out + j, d);
+            total = sc_lanes(total, L, SumOp());
+            inv = total == 0 ? 0.0f : 1.0f / total;
+            c = have ? g * (__builtin_amdgcn_exp2f((xi - m) * SC_LOG2E) * inv) : 0.0f;
+            all = inv * sc_lanes(c, L, SumOp());
+        } else {
+            const float w = sc_chosen_share(xi, have, a.sigmoid, a.renorm, L);
+            c = w * (g - (a.renorm ? sc_lanes(w * g, L, SumOp()) : 0.0f));
+            if (a.sigmoid) c *= xi > 0 ? expf(-xi) / (1 + expf(-xi)) : 1 / (1 + expf(xi));  // 1 - p
         }
+        pd_wave_sync();
+        if (have) unsafeAtomicAdd(acc + idx, c);
+        pd_wave_sync();
+        typename X::E* out = (typename X::E*)a.out + (on ? r : 0) * a.out_stride;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const int at = (v * L + l) * V;
+            if (!on || at >= E) continue;
+            float d[V];
+#pragma unroll
+            for (int e = 0; e < V; e += 4) *(float4*)(d + e) = *(const float4*)(acc + at + e);
+            if constexpr (DENSE) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) d[e] -= f[v * V + e] * all;
+            }
+            if (at + V <= E) {
+                sc_store<X>(out + at, X::pack(d));
+            } else {
+#pragma unroll
+                for (int e = 0; e < V; ++e)
+                    if (at + e < E) X::put(out + at + e, d[e]);
+            }
+        }
+        pd_wave_sync();  // the next rows' zeroes
     }
 }
 
@@ -1471,16 +1510,6 @@ static int sc_check_grad(const char* fn, const void* x, int dtype, int64_t rows,
         return sc_fail(fn, "grad overlaps the logits without being them");
     return PD_OK;
 }
-
-#define SC_BY_TYPE(dtype, kernel, grid, stream, args)                                                          \
-    do {                                                                                                       \
-        if ((dtype) == PD_F32)                                                                                 \
-            hipLaunchKernelGGL((kernel<F32>), dim3(grid), dim3(SC_WG), 0, (hipStream_t)(stream), args);      \
-        else if ((dtype) == PD_BF16)                                                                           \
-            hipLaunchKernelGGL((kernel<BF16>), dim3(grid), dim3(SC_WG), 0, (hipStream_t)(stream), args); \
-        else                                                                                                   \
-            hipLaunchKernelGGL((kernel<F16>), dim3(grid), dim3(SC_WG), 0, (hipStream_t)(stream), args);   \
-    } while (0)
 
 // Lanes to a row of up to SC_WAVE_COLS columns: the fewest with at most 32 scores to a lane, as long as that leaves
 // SC_ROW_WAVES wavefronts, four to a SIMD, and as the lanes' maxima bound the alternatives well.
@@ -1722,6 +1751,30 @@ extern "C" int pd_route_experts(const void* logits, int dtype, int64_t rows, int
     return sc_launched(fn);
 }
 
+template <typename X, int NV>
+static void sc_launch_route_grad_nv(const RouteGradArgs& a, hipStream_t stream) {
+    const int64_t rows_wg = 64 / a.lanes * SC_WAVES;
+    const dim3 grid(sc_grid((a.rows + rows_wg - 1) / rows_wg)), wg(SC_WG);
+    if (!a.sigmoid && !a.renorm)
+        hipLaunchKernelGGL((k_route_grad<X, NV, true>), grid, wg, 0, stream, a);
+    else
+        hipLaunchKernelGGL((k_route_grad<X, NV, false>), grid, wg, 0, stream, a);
+}
+
+template <typename X>
+static void sc_launch_route_grad(RouteGradArgs& a, hipStream_t stream) {
+    // A 16-byte piece of the row to a lane, a lane to every chosen expert; 16 experts to a lane at most (the LDS rows).
+    a.lanes = sc_pow2(a.top);
+    while (a.lanes < 64 && a.lanes * X::V < a.experts) a.lanes *= 2;
+    const int pieces = (a.experts + a.lanes * X::V - 1) / (a.lanes * X::V);
+    if (pieces <= 1)
+        sc_launch_route_grad_nv<X, 1>(a, stream);
+    else if (pieces <= 2)
+        sc_launch_route_grad_nv<X, 2>(a, stream);
+    else
+        sc_launch_route_grad_nv<X, 16 / X::V>(a, stream);
+}
+
 extern "C" int pd_route_experts_grad(const void* logits, int dtype, int64_t rows, int64_t experts, int64_t row_stride,
                                      const int32_t* index, const float* grad_weights, int score, int top, int renormalise,
                                      float scale, void* grad, int64_t grad_stride, void* stream) {
@@ -1734,6 +1787,11 @@ extern "C" int pd_route_experts_grad(const void* logits, int dtype, int64_t rows
     if (sc_check_grad(fn, logits, dtype, rows, experts, row_stride, grad, grad_stride)) return PD_E_INVALID;
     RouteGradArgs a = {logits, rows, row_stride, (int)experts, top, score == PD_SCORE_SIGMOID, renormalise != 0, scale,
                        index, grad_weights, grad, grad_stride};
-    SC_BY_TYPE(dtype, k_route_grad, sc_grid((rows + 3) / 4), stream, a);
+    if (dtype == PD_F32)
+        sc_launch_route_grad<F32>(a, (hipStream_t)stream);
+    else if (dtype == PD_BF16)
+        sc_launch_route_grad<BF16>(a, (hipStream_t)stream);
+    else
+        sc_launch_route_grad<F16>(a, (hipStream_t)stream);
     return sc_launched(fn);
 }
