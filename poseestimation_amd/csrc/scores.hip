@@ -854,17 +854,20 @@ __device__ __forceinline__ GradRow sc_grad_row(const LogprobGradArgs& a, int64_t
 
 // The gradient of NV vectors of V columns, vector u at at0 + u * step, from the scores f, in their place.
 template <typename X, int NV>
-__device__ __forceinline__ void sc_grad_values(const LogprobGradArgs& a, const GradRow& q, int n, float* f, int at0, int step,
-                                               int begin, int end) {
+__device__ __forceinline__ void sc_grad_values(const GradRow& q, float* f, int at0, int step, int begin, int end) {
     constexpr int V = X::V;
 #pragma unroll
     for (int i = 0; i < NV * V; ++i) {
         const float t = fmaf(f[i] - q.base, SC_LOG2E, -q.log2_sum);
         f[i] = -__builtin_amdgcn_exp2f(t) * fmaf(q.c1, sc_floor_t(t), q.c0);
     }
-    for (int k = 0; k < a.n_tok; ++k) {
+    // the tokens whose column one of this wavefront's lanes holds: piece (tok - begin) / V goes to lane (..) mod 64, of
+    // wavefront (..) / 64 mod the number of them (step / (64 V))
+    const int piece = (q.tok - begin) / V, wave = (at0 - begin) / (64 * V);
+    uint64_t mine = __ballot(q.tok >= begin && q.tok < end && (piece / 64) % (step / (64 * V)) == wave);
+    for (; mine; mine &= mine - 1) {
+        const int k = __ffsll((unsigned long long)mine) - 1;
         const int tok = __builtin_amdgcn_readlane(q.tok, k);
-        if (tok < begin || tok >= end) continue;
         const float g = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(q.g), k));
 #pragma unroll
         for (int i = 0; i < NV * V; ++i)
@@ -899,7 +902,7 @@ __global__ __launch_bounds__(SC_WG) void k_token_logprobs_grad_wave(LogprobGradA
 #pragma unroll
         for (int u = 0; u < NV; ++u) sc_read<X>(x, (u * 64 + lane) * V, n, f + u * V);
         const GradRow q = sc_grad_row(a, r, n, lane);
-        sc_grad_values<X, NV>(a, q, n, f, lane * V, 64 * V, 0, a.cols);
+        sc_grad_values<X, NV>(q, f, lane * V, 64 * V, 0, a.cols);
 #pragma unroll
         for (int u = 0; u < NV; ++u) sc_grad_store<X>(out, (u * 64 + lane) * V, n, a.cols, q.empty, f + u * V);
     }
@@ -931,7 +934,7 @@ __global__ __launch_bounds__(SC_WG) void k_token_logprobs_grad_block(LogprobGrad
             for (int u = 0; u < NV; ++u) sc_read<X>(x, at0 + (u * SC_WG + t) * V, n, f + u * V);
         }
         const GradRow q = sc_grad_row(a, r, n, t & 63);
-        sc_grad_values<X, NV>(a, q, n, f, at0 + t * V, SC_WG * V, at0, at0 + SC_CHUNK);
+        sc_grad_values<X, NV>(q, f, at0 + t * V, SC_WG * V, at0, at0 + SC_CHUNK);
         if (whole && !q.empty) {
 #pragma unroll
             for (int u = 0; u < NV; ++u) sc_store<X>(out + at0 + (u * SC_WG + t) * V, X::pack(f + u * V));
@@ -1331,11 +1334,12 @@ __global__ __launch_bounds__(SC_WG) void k_route(RouteArgs a) {
         K mine = best[0];
 #pragma unroll
         for (int k = 1; k < KP; ++k) mine = l == k ? best[k] : mine;
-        const int idx = bad ? -1 : Key::place(mine);
+        int idx = bad ? -1 : Key::place(mine);
         if constexpr (!CLOSE) {
             sc_route_put(a, r, l, L, on, idx, Key::score(mine), m, total);
         } else {
             if (biased) {
+                bool redo = false;  // the list's order, or its end, is open
                 // Two neighbours in the list that are too close: in order if they are equal by logit and bias.
                 K last = best[0];
                 uint32_t close = 0;
@@ -1348,7 +1352,7 @@ __global__ __launch_bounds__(SC_WG) void k_route(RouteArgs a) {
                 while (__any(close != 0)) {  // lane k of the row holds the k-th place
                     const int k = close ? __ffs((int)close) - 1 : 0, p0 = __shfl(idx, first + k), p1 = __shfl(idx, first + k + 1);
                     if (close)
-                        again |= sc_logit(a.x, a.dtype, row * a.stride + p0) != sc_logit(a.x, a.dtype, row * a.stride + p1) ||
+                        redo |= sc_logit(a.x, a.dtype, row * a.stride + p0) != sc_logit(a.x, a.dtype, row * a.stride + p1) ||
                                  a.bias[p0] != a.bias[p1];
                     close &= close - 1;
                 }
@@ -1364,8 +1368,53 @@ __global__ __launch_bounds__(SC_WG) void k_route(RouteArgs a) {
                     for (; near; near &= near - 1) {
                         const int j = __ffs((int)near) - 1;
                         if (j < have)
-                            again |= sc_logit(a.x, a.dtype, row * a.stride + place + j) != xl || a.bias[place + j] != bl;
+                            redo |= sc_logit(a.x, a.dtype, row * a.stride + place + j) != xl || a.bias[place + j] != bl;
                     }
+                }
+                redo = (__ballot(redo) & row_lanes) != 0;
+                again |= redo && !a.sigmoid;
+                if (a.sigmoid && __any(redo)) {
+                    // The experts that can be among the first `top` (not below the last one by more than the error): their
+                    // scores in float64, and their ranks among themselves.
+                    struct Cand {
+                        double by;
+                        int place;
+                    };
+                    Cand* cand = (Cand*)by[wave] + first / L * (2 * L);  // 64 / L rows of 2 L: 2 KB of the 8
+                    uint32_t take = 0;
+#pragma unroll
+                    for (int j = EPL - 1; j >= 0; --j) take = take + take + (s[j] >= edge - off);
+                    take = redo && kept ? take & (uint32_t)((1ull << have) - 1) : 0;
+                    const int count = sc_lanes(__popc(take), L, SumOp());
+                    const bool mend = redo && count <= 2 * L && fabsf(edge) < INFINITY;
+                    again |= redo && !mend;
+                    int to = __popc(take);  // an exclusive scan over the row's lanes
+                    for (int d = 1; d < L; d <<= 1) {
+                        const int o = __shfl_up(to, d, L);
+                        if (l >= d) to += o;
+                    }
+                    to -= __popc(take);
+                    if (mend)
+                        for (; take; take &= take - 1) cand[to++].place = place + __ffs((int)take) - 1;
+                    pd_wave_sync();
+                    if (mend)
+                        for (int i = l; i < count; i += L) {
+                            const int at = cand[i].place;
+                            const double v = 1 / (1 + exp(-(double)sc_logit(a.x, a.dtype, row * a.stride + at))) + (double)a.bias[at];
+                            cand[i].by = v >= -1e300 ? v : -1e300;
+                        }
+                    pd_wave_sync();
+                    int* order = (int*)(by[wave] + 2 * 64 * sizeof(Cand) / sizeof(double)) + first;
+                    if (mend)
+                        for (int i = l; i < count; i += L) {
+                            int rank = 0;
+                            for (int k = 0; k < count; ++k)
+                                rank += cand[k].by > cand[i].by || (cand[k].by == cand[i].by && cand[k].place < cand[i].place);
+                            if (rank < L) order[rank] = cand[i].place;
+                        }
+                    pd_wave_sync();
+                    if (mend) idx = l < a.top ? order[l] : -1;
+                    pd_wave_sync();  // the next rows go to the same place
                 }
             }
             uint64_t todo = __ballot(again && on && !bad);
@@ -1763,9 +1812,10 @@ static void sc_launch_route_grad_nv(const RouteGradArgs& a, hipStream_t stream) 
 
 template <typename X>
 static void sc_launch_route_grad(RouteGradArgs& a, hipStream_t stream) {
-    // A 16-byte piece of the row to a lane, a lane to every chosen expert; 16 experts to a lane at most (the LDS rows).
+    // A 16-byte piece of the row to a lane, two where there are many rows, and a lane to every chosen expert; 16 experts to
+    // a lane at most (the LDS rows).
     a.lanes = sc_pow2(a.top);
-    while (a.lanes < 64 && a.lanes * X::V < a.experts) a.lanes *= 2;
+    while (a.lanes < 64 && a.lanes * X::V * (a.rows >= SC_ROUTE_WAVES * 8 ? 2 : 1) < a.experts) a.lanes *= 2;
     const int pieces = (a.experts + a.lanes * X::V - 1) / (a.lanes * X::V);
     if (pieces <= 1)
         sc_launch_route_grad_nv<X, 1>(a, stream);
