@@ -421,6 +421,23 @@ def test_route_orders_near_scores_as_float64_does():
                 _check_route(x[r:r + 16], 8, bias=bias, score=score, groups=groups, top_groups=top_groups, group_score='max')
 
 
+def test_route_orders_a_few_near_scores_in_and_around_the_list():
+    """Six experts whose scores differ by less than float32 tells, at places that put them inside the list, at its end and
+    beyond it, the other experts well apart."""
+    gen = torch.Generator().manual_seed(21)
+    for experts, groups, top_groups, top in ((64, 1, 1, 8), (256, 8, 4, 8), (256, 1, 1, 6), (160, 1, 1, 6), (1024, 1, 1, 8), (48, 1, 1, 2)):
+        for above in (0, 1, 3, 5, 7, 9):
+            for score in ('sigmoid', 'softmax'):
+                x = (torch.randn(20, experts, generator=gen) * 0.8).cuda()
+                p = torch.from_numpy(ref.probability(_np(x)[7], score))
+                # apart by 2e-3, then `above` of them first and six to one value
+                target = 0.25 + 2e-3 * torch.randperm(experts, generator=gen).double()
+                order = target.argsort(descending=True)
+                target[order[above:above + 6]] = target[order[above]].item()
+                bias = (target - p).float().cuda()
+                _check_route(x, top, bias=bias, score=score, groups=groups, top_groups=top_groups)
+
+
 @pytest.mark.parametrize('dtype', list(TYPES))
 def test_route_of_strided_misaligned_and_expanded_rows(dtype):
     store = torch.full((40, 300), math.nan, dtype=TYPES[dtype], device='cuda')
