@@ -537,8 +537,8 @@ __global__ __launch_bounds__(SC_WG) void k_token_logprobs_rows(LogprobArgs a) {
 // Chunks of WG * 32 columns, 32 to a thread in 16-byte loads.  With many rows: 64 or 256 threads, and workgroups enough on
 // a CU to keep the loads coming while others reduce; bound by the memory (4096 x 131072 bfloat16 with five alternatives:
 // 196 us, 5.5 TB/s).  With few long rows: 1024 threads that load a chunk while they add the one before; bound by
-// instruction issue on the one CU (131072 columns 9 us) and by the latency of the steps behind the last load.  Rows that would
-// take one CU longer are cut into slices, joined by k_token_logprobs_join.
+// instruction issue on the one CU (131072 columns 9 us) and by the latency of the steps behind the last load.  Still fewer
+// long rows are cut into slices, joined by k_token_logprobs_join.
 
 #define SC_PER_THREAD 32
 #define SC_MAX_CHUNKS(WG) ((WG) == 1024 ? 8 : 16)
@@ -755,11 +755,16 @@ __global__ __launch_bounds__(WG) void k_token_logprobs_block(LogprobArgs a) {
     }
 }
 
-// The slices of a row: their statistics by the rule above, their alternatives (each slice's in order) merged.  With
-// j = ceil(top / slices) the least of the slices' j-th keys has at least `top` keys from it on.
+// The slices of a row: their statistics by the rule above, their alternatives (each slice's in order) merged.  If the j-th keys
+// of q slices reach a bound, at least q j keys do; the smallest j with q j >= top (q of the slices) makes the bound a close one:
+// of 256 slices with 64 keys each some 75 reach the 64th largest of the first keys.  At most 256 slices (sc_cut).
+#define SC_AHEAD 4
+
 template <typename X>
 __global__ __launch_bounds__(SC_WG) void k_token_logprobs_join(LogprobArgs a) {
     __shared__ uint64_t cand[SC_CAND], wave_key[SC_WAVES];
+    __shared__ uint64_t heads[SC_WG];
+    __shared__ uint32_t from;
     __shared__ Stat wave_stat[SC_WAVES];
     __shared__ int n_cand;
     const int t = threadIdx.x;
@@ -767,6 +772,15 @@ __global__ __launch_bounds__(SC_WG) void k_token_logprobs_join(LogprobArgs a) {
         const typename X::E* x = (const typename X::E*)a.x + r * a.stride;
         const int n = sc_width(a.widths, r, a.cols);
         const RowToken tok = sc_row_token<X>(a, r, x, n, t);
+        // everything the row needs is asked for at once: it comes from other XCDs' workgroups, by way of the memory
+        const uint64_t* keys = a.part_keys + r * a.slices * a.top;
+        const int total = a.slices * a.top;
+        const int j = a.top ? (a.top + a.slices - 1) / a.slices : 1, reach = (a.top + j - 1) / j;
+        uint64_t ahead[SC_AHEAD];
+#pragma unroll
+        for (int i = 0; i < SC_AHEAD; ++i) ahead[i] = t + i * SC_WG < total ? keys[t + i * SC_WG] : 0;
+        uint64_t head = 0;  // two slices without a j-th key differ by the thread
+        if (a.top && t < a.slices) heads[t] = head = (keys[t * a.top + j - 1] >> 32 << 32) | t;
         Stat st = {-INFINITY, 0, 0};
         for (int i = t; i < a.slices; i += SC_WG) {
             Stat o = a.part[r * a.slices + i];
@@ -783,18 +797,17 @@ __global__ __launch_bounds__(SC_WG) void k_token_logprobs_join(LogprobArgs a) {
         if (a.top && (q.bad || q.empty)) {
             if (t < a.top) sc_put_top(a, r, t, q.bad ? 0 : sc_key(-INFINITY, t), q);
         } else if (a.top) {
-            const uint64_t* keys = a.part_keys + r * a.slices * a.top;
-            const int total = a.slices * a.top, j = (a.top + a.slices - 1) / a.slices;
-            uint64_t from = ~0ull;
-            for (int i = t; i < a.slices; i += SC_WG) from = MinOp()(from, keys[i * a.top + j - 1]);
-            from = sc_block<SC_WG>(from, MinOp(), wave_key);
-            for (int i = t; i < total; i += SC_WG) {
-                const uint64_t key = keys[i];
-                if (key && key >= from) {
+            if (t < a.slices && sc_rank(heads, a.slices, head) == reach - 1) from = (uint32_t)(head >> 32);
+            __syncthreads();
+            const auto collect = [&](uint64_t key) {
+                if (key && (uint32_t)(key >> 32) >= from) {
                     const int to = atomicAdd(&n_cand, 1);
                     if (to < SC_CAND) cand[to] = key;
                 }
-            }
+            };
+#pragma unroll
+            for (int i = 0; i < SC_AHEAD; ++i) collect(ahead[i]);
+            for (int i = t + SC_AHEAD * SC_WG; i < total; i += SC_WG) collect(keys[i]);
             __syncthreads();
             const int have = n_cand;
             if (have <= SC_CAND) {
@@ -805,13 +818,12 @@ __global__ __launch_bounds__(SC_WG) void k_token_logprobs_join(LogprobArgs a) {
                 }
                 if (t >= have && t < a.top) sc_put_top(a, r, t, 0, q);
             } else {
-                uint64_t prev = ~0ull;
-                for (int k = 0; k < a.top; ++k) {
-                    uint64_t best = 0;
-                    for (int i = t; i < total; i += SC_WG)
-                        if (keys[i] < prev && keys[i] > best) best = keys[i];
-                    prev = sc_block<SC_WG>(best, MaxOp(), wave_key);
-                    if (t == 0) sc_put_top(a, r, k, prev, q);
+                // too many equal scores: the largest of the slices' next keys, one after the other
+                uint64_t next = t < a.slices ? keys[t * a.top] : 0;
+                for (int k = 0, at = 0; k < a.top; ++k) {
+                    const uint64_t best = sc_block<SC_WG>(next, MaxOp(), wave_key);
+                    if (t == 0) sc_put_top(a, r, k, best, q);
+                    if (next == best && best) next = ++at < a.top ? keys[t * a.top + at] : 0;
                 }
             }
         }
@@ -1585,11 +1597,13 @@ static int sc_row_lanes(int64_t rows, int64_t cols, int top) {
 // threads: 8192 x 4096 22 / 43 / 224 us, 16 x 4096 6.1 / 6.2 / 8.1, 4096 x 16384 28 / 31 / 117, 1400 x 16384 17 / 15 / 45,
 // 200 x 16384 10.7 / 6.8 / 8.6, 4096 x 131072 233 / 214 / 261, 255 x 131072 25 / 24 / 19.  So: one wavefront for rows of up to
 // 4096 columns, and up to 32768 where there are eight for every CU (it waits for no other at a row's end); 1024 threads for
-// long rows that leave CUs idle, in slices of at least SC_SLICE_COLS, as many as there are CUs for (a CU takes 9 us for that
-// many, about what the join of slices costs with its launch); 256 otherwise.  More than 32 alternatives need 256 parts.
+// long rows that leave CUs idle; 256 otherwise.  More than 32 alternatives need 256 parts.
+// A row alone keeps one CU busy for 9 us per 131072 columns, and the join of slices costs 4 us: where few rows leave CUs for
+// eight slices of SC_SLICE_COLS they are cut into as many as there are CUs for (1 x 131072 15.8 -> 12.5 us, 1 x 1000000 float32
+// 21 -> 14; 100 x 131072 in two would go from 15 to 17).
 #define SC_WAVE_COLS 2048
 #define SC_CUS 256
-#define SC_SLICE_COLS (128 << 10)
+#define SC_SLICE_COLS 16384
 
 struct Cut {
     int wg, slices, slice_cols;
@@ -1597,14 +1611,14 @@ struct Cut {
 
 static Cut sc_cut(int64_t rows, int64_t cols, int top) {
     Cut c;
+    int64_t want = SC_CUS / rows < cols / SC_SLICE_COLS ? SC_CUS / rows : cols / SC_SLICE_COLS;
+    if (want < 8) want = 1;
     if (top <= 32 && (cols <= 4096 || (cols <= 32768 && rows >= 8 * SC_CUS)))
         c.wg = 64;
     else
-        c.wg = rows < SC_CUS && cols > 32768 ? 1024 : SC_WG;
+        c.wg = rows < SC_CUS && cols > 32768 && want == 1 ? 1024 : SC_WG;
     const int64_t chunk = (int64_t)c.wg * SC_PER_THREAD, chunks = (cols + chunk - 1) / chunk;
-    int64_t want = c.wg < 1024 ? 1 : SC_CUS / rows;
-    const int64_t most = cols / SC_SLICE_COLS, least = (chunks + SC_MAX_CHUNKS(c.wg) - 1) / SC_MAX_CHUNKS(c.wg);
-    if (want > most) want = most;
+    const int64_t least = (chunks + SC_MAX_CHUNKS(c.wg) - 1) / SC_MAX_CHUNKS(c.wg);  // what the segments' LDS holds
     if (want < least) want = least;
     const int64_t each = (chunks + want - 1) / want;
     c.slices = (int)((chunks + each - 1) / each);

@@ -111,22 +111,24 @@ def token_logprobs(logits, tokens=None, top=0, widths=None):
         n_tok = shape[1] if len(shape) == 2 else 1
     if widths is not None:
         widths = _like(widths, 'widths', torch.int32, ((rows,),), dev)
-    # one allocation for what a call returns, cut into the parts
+    # one allocation for what a call returns, cut into the parts, behind the workspace where that is small
     k = max(top, 0)
-    store = torch.empty(rows * (n_tok + 2 * k + 4), dtype=torch.float32, device=dev)
-    entropy = store.as_strided((rows,), (1,))
-    stats = store.as_strided((rows, 3), (3, 1), rows)
-    logp = top_logp = top_index = ws = None
-    at = 4 * rows
+    ws_bytes = _ffi.lib().pd_token_logprobs_workspace(code, rows, columns, top)
+    at = ws_bytes // 4 if ws_bytes <= 1 << 18 else 0
+    store = torch.empty(at + rows * (n_tok + 2 * k + 4), dtype=torch.float32, device=dev)
+    ws = None
+    if ws_bytes:
+        ws = store if at else torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    entropy = store.as_strided((rows,), (1,), at)
+    stats = store.as_strided((rows, 3), (3, 1), at + rows)
+    logp = top_logp = top_index = None
+    at += 4 * rows
     if k:
         top_logp = store.as_strided((rows, k), (k, 1), at)
         top_index = store.view(torch.int32).as_strided((rows, k), (k, 1), at + rows * k)
         at += 2 * rows * k
     if shape is not None:
         logp = store.as_strided(shape, (n_tok, 1) if len(shape) == 2 else (1,), at)
-    ws_bytes = _ffi.lib().pd_token_logprobs_workspace(code, rows, columns, top)
-    if ws_bytes:
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
     _call('pd_token_logprobs', dev, logits.data_ptr(), code, rows, columns, stride, _address(widths), _address(tokens), n_tok,
           top, _address(logp), entropy.data_ptr(), stats.data_ptr(), _address(top_logp), _address(top_index),
           _address(ws), ws_bytes)

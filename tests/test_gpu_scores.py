@@ -165,6 +165,20 @@ def test_alternatives_that_all_lie_in_few_lanes(cols, period):
     _check_many(x.bfloat16(), None, 50, times=128)
 
 
+@pytest.mark.parametrize('cols, top', [(131072, 64), (600000, 20), (1500000, 64)])
+def test_alternatives_of_long_rows_with_equal_scores(cols, top):
+    """Slices whose keys are all alike: constant rows, few scores that are not masked, two values, whole steps."""
+    for fill, some in ((1.0, None), (-math.inf, 5), (-math.inf, 300), (0.0, 17), (-3e38, 3)):
+        x = torch.full((2, cols), fill, dtype=torch.bfloat16, device='cuda')
+        if some:
+            at = torch.randperm(cols, generator=torch.Generator().manual_seed(some))[:some].cuda()
+            x[0, at] = 2.0
+            x[1, at] = torch.arange(some, device='cuda').bfloat16()
+        _check_logprobs(x, _tokens(2, cols, 2), top)
+    x = torch.randint(0, 4, (2, cols), generator=torch.Generator().manual_seed(cols)).to(torch.bfloat16).cuda()
+    _check_logprobs(x, None, top, torch.tensor([cols, cols // 3], dtype=torch.int32, device='cuda'))
+
+
 @pytest.mark.parametrize('cols', [40, 656, 5000, 20000])
 def test_logprobs_of_ragged_rows(cols):
     x = _rows(11, cols, 'bf16', seed=5)
