@@ -976,9 +976,9 @@ __global__ __launch_bounds__(SC_WG) void k_token_logprobs_grad_block(LogprobGrad
 // sc_route_row for it, a wavefront to the row).  The same goes for the groups.
 //
 // A row belongs to L lanes (a power of two, whole groups to whole lanes), a lane holds EPL consecutive experts of one
-// group, a wavefront 64 / L rows.  A score and its place are one floating-point number, the place in mantissa bits that
-// the score does not use, so that one v_max orders both and no two are equal: bfloat16 and float16 logits leave 13 bits
-// of a float32, all else goes into a float64 (its v_max issues at the same rate).  A lane sorts its experts KP at a time by
+// group, a wavefront 64 / L rows.  A score and its place are one number, the place in mantissa bits that the score does not
+// use, so that one v_max orders both and no two are equal: bfloat16 and float16 logits leave 13 bits of 32, all else goes
+// into a float64 (whose v_max issues at the same rate).  A lane sorts its experts KP at a time by
 // a bitonic network, keeps the best KP, and the lanes merge theirs in log2 L exchanges.  Bound by instruction issue.
 
 struct RouteArgs {
@@ -1113,8 +1113,8 @@ __device__ __forceinline__ void sc_route_row(const RouteArgs& a, int64_t r, int 
 
 __device__ __forceinline__ double sc_hi(double a, double b) { return fmax(a, b); }
 __device__ __forceinline__ double sc_lo(double a, double b) { return fmin(a, b); }
-__device__ __forceinline__ float sc_hi(float a, float b) { return fmaxf(a, b); }
-__device__ __forceinline__ float sc_lo(float a, float b) { return fminf(a, b); }
+__device__ __forceinline__ uint32_t sc_hi(uint32_t a, uint32_t b) { return a > b ? a : b; }
+__device__ __forceinline__ uint32_t sc_lo(uint32_t a, uint32_t b) { return a < b ? a : b; }
 
 template <typename K>
 __device__ __forceinline__ void sc_exchange(K& a, K& b) {  // the larger first
@@ -1161,28 +1161,21 @@ __device__ __forceinline__ void sc_merge_across(K* a) {
     sc_merge<N>(a, q);
 }
 
-// Score and place as one number.  Of two equal scores the one of the lower place is the larger: where the number is
-// negative the one with the smaller magnitude.  -inf (float64: and NaN) comes behind every finite score.
+// Score and place as one number.  Of two equal scores the one of the lower place is the larger: where a float64 is negative
+// the one with the smaller magnitude.  -inf (float64: and NaN) comes behind every finite score, NONE behind that.
 #define SC_PLACES (PD_MAX_EXPERTS - 1)
-struct Key32 {  // of a bfloat16 or float16 value: its float32 has 13 bits to spare, and no finite one reaches SC_INF32
-    typedef float K;
-    static constexpr uint32_t SC_INF32 = 0x7f7ffc00u;
-    static __device__ __forceinline__ K make(float s, int place) {
-        const float f = __builtin_amdgcn_fmed3f(s + 0.0f, -__uint_as_float(SC_INF32), __uint_as_float(SC_INF32));
-        const uint32_t u = __float_as_uint(f);
-        return __uint_as_float(u | ((uint32_t)place ^ (~(uint32_t)((int32_t)u >> 31) & SC_PLACES)));
-    }
-    static __device__ __forceinline__ int place(K key) {
-        const uint32_t u = __float_as_uint(key);
-        return (int)((u ^ ~(uint32_t)((int32_t)u >> 31)) & SC_PLACES);
-    }
+struct Key32 {  // of a bfloat16 or float16 value: the order of its float32, whose lowest 13 bits are the same for all
+    typedef uint32_t K;
+    static constexpr K NONE = 0;
+    static __device__ __forceinline__ K make(float s, int place) { return (sc_order(s) & ~(uint32_t)SC_PLACES) | (SC_PLACES - place); }
+    static __device__ __forceinline__ int place(K key) { return SC_PLACES - (int)(key & SC_PLACES); }
     static __device__ __forceinline__ float score(K key) {
-        const uint32_t u = __float_as_uint(key) & ~(uint32_t)SC_PLACES, mag = u & 0x7fffffffu;
-        return __uint_as_float(mag >= SC_INF32 ? (u & 0x80000000u) | 0x7f800000u : u);
+        return sc_unorder(key >> 31 ? key & ~(uint32_t)SC_PLACES : key | SC_PLACES);
     }
 };
 struct Key64 {
     typedef double K;
+    static constexpr K NONE = -INFINITY;
     static __device__ __forceinline__ K make(float s, int place) {
         const double d = fmin(fmax((double)(s + 0.0f), -0x1p1000), 0x1p1000);
         const uint64_t u = __double_as_longlong(d);
@@ -1331,12 +1324,12 @@ __global__ __launch_bounds__(SC_WG) void k_route(RouteArgs a) {
                 for (int j = 0; j < B; ++j) v[j] = Key::make(CLOSE && biased ? s[b + j] : x[b + j], place + b + j);
                 if (!full) {
 #pragma unroll
-                    for (int j = 0; j < B; ++j) v[j] = b + j < have ? v[j] : -INFINITY;
+                    for (int j = 0; j < B; ++j) v[j] = b + j < have ? v[j] : Key::NONE;
                 }
                 sc_sort<B>(v);
                 if (b == 0) {
 #pragma unroll
-                    for (int j = 0; j < KP; ++j) best[j] = j < B ? v[j < B ? j : 0] : -INFINITY;
+                    for (int j = 0; j < KP; ++j) best[j] = j < B ? v[j < B ? j : 0] : Key::NONE;
                 } else if constexpr (B == KP) {
                     sc_merge<KP>(best, v);
                 }
@@ -1344,7 +1337,7 @@ __global__ __launch_bounds__(SC_WG) void k_route(RouteArgs a) {
         }
         if (a.groups > 1) {
 #pragma unroll
-            for (int j = 0; j < KP; ++j) best[j] = kept ? best[j] : -INFINITY;
+            for (int j = 0; j < KP; ++j) best[j] = kept ? best[j] : Key::NONE;
         }
         if (L > 1) sc_merge_across<KP, 1>(best);
         if (L > 2) sc_merge_across<KP, 2>(best);
