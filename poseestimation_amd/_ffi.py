@@ -17,6 +17,7 @@ MEM_HOST, MEM_DEVICE = 0, 1
 F32, F64, U8, BF16, F16 = 0, 1, 2, 3, 4
 SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
 GROUP_MAX, GROUP_TOP2 = 0, 1
+MAX_ALTERNATIVES, MAX_ROUTES = 64, 32
 IMPL_FAST, IMPL_SIMPLE, IMPL_STREAM = 0, 1, 2
 
 EXPORTS = ['pd_create', 'pd_destroy', 'pd_last_error', 'pd_version', 'pd_set_mode', 'pd_set_impl',

@@ -49,7 +49,8 @@ def _like(x, name, dtype, shapes, device):
     if x.dtype != dtype:
         if x.is_floating_point() != dtype.is_floating_point or x.dtype == torch.bool or x.is_complex():
             raise ValueError('%s must hold %s, got %s' % (name, 'numbers' if dtype.is_floating_point else 'whole numbers', x.dtype))
-        x = x.to(dtype)
+        # (int32: a larger number stays out of every range)
+        x = x.clamp(-1, 0x7fffffff).to(dtype) if dtype == torch.int32 else x.to(dtype)
     return x if x.is_contiguous() else x.contiguous()
 
 
@@ -60,19 +61,18 @@ def _tokens(tokens, rows, device):
     return _like(tokens, 'tokens', torch.int64, (shape,), device), shape
 
 
-def _call(fn, device, *args):
-    """One call of the library on the current stream of ``device``."""
-    L = _ffi.lib()
-    # (the stream's address itself: making a Stream object of it takes longer than the rest of a small call's checks)
-    stream = torch._C._cuda_getCurrentRawStream(device.index)
-    if torch.cuda.current_device() != device.index:
-        with torch.cuda.device(device):
-            rc = getattr(L, fn)(*args, stream)
-    else:
-        rc = getattr(L, fn)(*args, stream)
-    if rc == _ffi.PD_OK:
-        return
-    msg = L.pd_last_error(None).decode()
+def _current(device):
+    """Whether ``device`` is the current one, which the library's calls work on."""
+    return torch.cuda.current_device() == device.index
+
+
+def _stream(device):
+    # (the stream's address itself: making a Stream object of it takes longer than the checks of a small call)
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _raise(rc):
+    msg = _ffi.lib().pd_last_error(None).decode()
     if rc == _ffi.PD_E_INVALID:
         raise ValueError(msg)
     raise RuntimeError('libposedecode error %d: %s' % (rc, msg))
@@ -105,17 +105,22 @@ def token_logprobs(logits, tokens=None, top=0, widths=None):
     -inf, entropy 0, alternatives 0, 1, .. .  A row that holds a NaN or +inf: NaN, alternatives -1."""
     code, rows, columns, stride = _rows(logits, 'logits')
     dev = logits.device
+    if not _current(dev):
+        with torch.cuda.device(dev):
+            return token_logprobs(logits, tokens, top, widths)
     n_tok, shape, top = 0, None, int(top)
+    if not 0 <= top <= min(_ffi.MAX_ALTERNATIVES, columns):
+        raise ValueError('top must be within 0..%d and the columns, got %d' % (_ffi.MAX_ALTERNATIVES, top))
     if tokens is not None:
         tokens, shape = _tokens(tokens, rows, dev)
         n_tok = shape[1] if len(shape) == 2 else 1
     if widths is not None:
         widths = _like(widths, 'widths', torch.int32, ((rows,),), dev)
     # one allocation for what a call returns, cut into the parts, behind the workspace where that is small
-    k = max(top, 0)
-    ws_bytes = _ffi.lib().pd_token_logprobs_workspace(code, rows, columns, top)
+    L = _ffi.lib()
+    ws_bytes = L.pd_token_logprobs_workspace(code, rows, columns, top)
     at = ws_bytes // 4 if ws_bytes <= 1 << 18 else 0
-    store = torch.empty(at + rows * (n_tok + 2 * k + 4), dtype=torch.float32, device=dev)
+    store = torch.empty(at + rows * (n_tok + 2 * top + 4), dtype=torch.float32, device=dev)
     ws = None
     if ws_bytes:
         ws = store if at else torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
@@ -123,15 +128,17 @@ def token_logprobs(logits, tokens=None, top=0, widths=None):
     stats = store.as_strided((rows, 3), (3, 1), at + rows)
     logp = top_logp = top_index = None
     at += 4 * rows
-    if k:
-        top_logp = store.as_strided((rows, k), (k, 1), at)
-        top_index = store.view(torch.int32).as_strided((rows, k), (k, 1), at + rows * k)
-        at += 2 * rows * k
+    if top:
+        top_logp = store.as_strided((rows, top), (top, 1), at)
+        top_index = store.view(torch.int32).as_strided((rows, top), (top, 1), at + rows * top)
+        at += 2 * rows * top
     if shape is not None:
         logp = store.as_strided(shape, (n_tok, 1) if len(shape) == 2 else (1,), at)
-    _call('pd_token_logprobs', dev, logits.data_ptr(), code, rows, columns, stride, _address(widths), _address(tokens), n_tok,
-          top, _address(logp), entropy.data_ptr(), stats.data_ptr(), _address(top_logp), _address(top_index),
-          _address(ws), ws_bytes)
+    rc = L.pd_token_logprobs(logits.data_ptr(), code, rows, columns, stride, _address(widths), _address(tokens), n_tok, top,
+                             _address(logp), entropy.data_ptr(), stats.data_ptr(), _address(top_logp), _address(top_index),
+                             _address(ws), ws_bytes, _stream(dev))
+    if rc:
+        _raise(rc)
     return TokenLogprobs(logp, entropy, top_logp, top_index, stats)
 
 
@@ -143,6 +150,9 @@ def token_logprobs_backward(logits, stats, tokens=None, grad_logp=None, grad_ent
     themselves are allowed."""
     code, rows, columns, stride = _rows(logits, 'logits')
     dev = logits.device
+    if not _current(dev):
+        with torch.cuda.device(dev):
+            return token_logprobs_backward(logits, stats, tokens, grad_logp, grad_entropy, widths, out)
     stats = _like(stats, 'stats', torch.float32, ((rows, 3),), dev)
     n_tok = 0
     if (tokens is None) != (grad_logp is None):
@@ -158,8 +168,11 @@ def token_logprobs_backward(logits, stats, tokens=None, grad_logp=None, grad_ent
     if widths is not None:
         widths = _like(widths, 'widths', torch.int32, ((rows,),), dev)
     out, out_stride = _grad_out(out, logits)
-    _call('pd_token_logprobs_grad', dev, logits.data_ptr(), code, rows, columns, stride, _address(widths), stats.data_ptr(),
-          _address(tokens), n_tok, _address(grad_logp), _address(grad_entropy), out.data_ptr(), out_stride)
+    rc = _ffi.lib().pd_token_logprobs_grad(logits.data_ptr(), code, rows, columns, stride, _address(widths), stats.data_ptr(),
+                                           _address(tokens), n_tok, _address(grad_logp), _address(grad_entropy), out.data_ptr(),
+                                           out_stride, _stream(dev))
+    if rc:
+        _raise(rc)
     return out
 
 
@@ -184,16 +197,24 @@ def route_experts(logits, top, score='softmax', bias=None, groups=1, top_groups=
     renormalised.  A row that holds a NaN (softmax: or +inf): weights NaN, index -1."""
     code, rows, experts, stride = _rows(logits, 'logits')
     dev = logits.device
+    if not _current(dev):
+        with torch.cuda.device(dev):
+            return route_experts(logits, top, score, bias, groups, top_groups, group_score, renormalise, scale)
     score = _score_code(_SCORES, score, 'score')
     group_score = _score_code(_GROUP_SCORES, group_score, 'group_score')
     if bias is not None:
         bias = _like(bias, 'bias', torch.float32, ((experts,),), dev)
     top, groups = int(top), int(groups)
     top_groups = groups if top_groups is None else int(top_groups)
-    weights = torch.empty((rows, max(top, 0)), dtype=torch.float32, device=dev)
-    index = torch.empty((rows, max(top, 0)), dtype=torch.int32, device=dev)
-    _call('pd_route_experts', dev, logits.data_ptr(), code, rows, experts, stride, _address(bias), score, groups, top_groups,
-          group_score, top, 1 if renormalise else 0, float(scale), weights.data_ptr(), index.data_ptr())
+    if not 1 <= top <= min(_ffi.MAX_ROUTES, experts):
+        raise ValueError('top must be within 1..%d and the experts, got %d' % (_ffi.MAX_ROUTES, top))
+    weights = torch.empty((rows, top), dtype=torch.float32, device=dev)
+    index = torch.empty((rows, top), dtype=torch.int32, device=dev)
+    rc = _ffi.lib().pd_route_experts(logits.data_ptr(), code, rows, experts, stride, _address(bias), score, groups, top_groups,
+                                     group_score, top, 1 if renormalise else 0, scale, weights.data_ptr(), index.data_ptr(),
+                                     _stream(dev))
+    if rc:
+        _raise(rc)
     return Routes(weights, index)
 
 
@@ -203,6 +224,9 @@ def route_experts_backward(logits, index, grad_weights, score='softmax', renorma
     counts twice.  ``out``: where to put it; the logits themselves are allowed."""
     code, rows, experts, stride = _rows(logits, 'logits')
     dev = logits.device
+    if not _current(dev):
+        with torch.cuda.device(dev):
+            return route_experts_backward(logits, index, grad_weights, score, renormalise, scale, out)
     score = _score_code(_SCORES, score, 'score')
     if not isinstance(index, torch.Tensor) or index.dim() != 2:
         raise ValueError('index must be a (rows, top) tensor of whole numbers')
@@ -210,6 +234,8 @@ def route_experts_backward(logits, index, grad_weights, score='softmax', renorma
     index = _like(index, 'index', torch.int32, ((rows, top),), dev)
     grad_weights = _like(grad_weights, 'grad_weights', torch.float32, ((rows, top),), dev)
     out, out_stride = _grad_out(out, logits)
-    _call('pd_route_experts_grad', dev, logits.data_ptr(), code, rows, experts, stride, index.data_ptr(),
-          grad_weights.data_ptr(), score, top, 1 if renormalise else 0, float(scale), out.data_ptr(), out_stride)
+    rc = _ffi.lib().pd_route_experts_grad(logits.data_ptr(), code, rows, experts, stride, index.data_ptr(), grad_weights.data_ptr(),
+                                          score, top, 1 if renormalise else 0, scale, out.data_ptr(), out_stride, _stream(dev))
+    if rc:
+        _raise(rc)
     return out
