@@ -441,7 +441,8 @@ int pd_token_logprobs(const void* logits, int dtype, int64_t rows, int64_t colum
 /* The gradient with respect to the logits, of their type, every column of every row:
  *   grad[r][j] = -p_j (sum_t grad_logp[r][t] + grad_entropy[r] (log p_j + entropy[r])) + sum over t with
  *   tokens[r][t] = j of grad_logp[r][t],   p_j = exp(x_j - m - log S) from stats.
- * Tokens that are not given contribute nothing; columns behind a row's width and empty rows get 0.
+ * Tokens that are not given contribute nothing, tokens that the row does not hold the first term only; columns
+ * behind a row's width and empty rows get 0.
  * grad_entropy may be NULL.  grad may be the logits themselves (same stride) or must not overlap them. */
 int pd_token_logprobs_grad(const void* logits, int dtype, int64_t rows, int64_t columns, int64_t row_stride,
                            const int32_t* widths, const float* stats, const int64_t* tokens, int n_tokens,

@@ -407,6 +407,28 @@ __device__ __forceinline__ uint32_t sc_kth(const uint32_t* o, int K) {
     return t;
 }
 
+// A number that exactly K of a row's scores f reach, one wavefront to the row, or the K-th largest itself where there are
+// equals; lo, hi: orders of which at least K scores reach the first, and none exceeds the second.
+template <int N>
+__device__ __forceinline__ float sc_kth_all(const float* f, int K, uint32_t lo, uint32_t hi) {
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    hi = __builtin_amdgcn_readfirstlane(hi);
+    if (lo == hi) return sc_unorder(hi);
+    const int bits = 32 - __clz(hi ^ lo);
+    uint32_t t = bits == 32 ? 0 : hi >> bits << bits;
+    for (int bit = bits - 1; bit >= 0; --bit) {
+        const uint32_t trial = t | 1u << bit;
+        if (trial > hi) continue;
+        const float at = sc_unorder(trial);
+        int count = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) count += __popcll(__ballot(f[i] >= at));
+        if (count >= K) t = trial;
+        if (count == K) break;
+    }
+    return sc_unorder(t > lo ? t : lo);
+}
+
 // ---- 16, 32 or 64 lanes to the row: up to 2048 columns, all of them in registers ----------------
 //
 // Bound by instruction issue and latency, not by memory: some ten instructions a score, and a few hundred for the
@@ -464,16 +486,24 @@ __global__ __launch_bounds__(SC_WG) void k_token_logprobs_rows(LogprobArgs a) {
         }
         // What reaches tau is marked without a branch, and the few are read again: N branches with a key each would take
         // 80 registers more.
-        uint32_t take = 0;
+        uint32_t take;
+        int count;
+        for (bool once = L == 64;; once = false) {
+            take = 0;
 #pragma unroll
-        for (int i = N - 1; i >= 0; --i) take = take + take + (f[i] >= tau);
-        if (__any(tau == -INFINITY)) {  // then what lies behind the row does, too
-            uint32_t valid = 0;
-            for (int u = 0; u < NV; ++u) valid |= ((1u << pd_clampi(n - (u * L + l) * V, 0, V)) - 1) << (u * V);
-            take &= valid;
+            for (int i = N - 1; i >= 0; --i) take = take + take + (f[i] >= tau);
+            if (__any(tau == -INFINITY)) {  // then what lies behind the row does, too
+                uint32_t valid = 0;
+                for (int u = 0; u < NV; ++u) valid |= ((1u << pd_clampi(n - (u * L + l) * V, 0, V)) - 1) << (u * V);
+                take &= valid;
+            }
+            if (!plain) take = 0;
+            count = sc_lanes(__popc(take), L, SumOp());
+            if (!once || count <= room) break;
+            // With many alternatives, or more than there are lanes in use, too many scores reach the lanes' bound (at 64 some
+            // 250 of 2048): it is taken on from there among all of them.
+            tau = sc_kth_all<N>(f, a.top, sc_order(tau), sc_order(st.m));
         }
-        if (!plain) take = 0;
-        int count = sc_lanes(__popc(take), L, SumOp());
         if (__any(count > room)) {
             // Too many scores equal to tau (a masked row, a constant one): of those the first that make up the number.
             uint32_t above = 0;
@@ -968,7 +998,6 @@ __global__ __launch_bounds__(SC_WG) void k_token_logprobs_grad_block(LogprobGrad
 }
 
 // ---- routing -------------------------------------------------------------------------------
-
 //
 // The order of the experts is that of float64 arithmetic, so that it does not depend on how a kernel forms its sums.
 // Without a bias it is the order of the logits, which float32 holds exactly.  With one, the scores p + bias are formed
@@ -1265,8 +1294,9 @@ __global__ __launch_bounds__(SC_WG) void k_route(RouteArgs a) {
                 const float inv = total == 0 ? 0.0f : 1.0f / total;
 #pragma unroll
                 for (int j = 0; j < EPL; ++j) s[j] *= inv;
-                // the largest p is 1 / total, and every p is off by at most (EPL + 40) u of it: the sum's EPL + 6 steps, the
-                // exponents' |t| 2^t, the exponential, the division; the difference of two by twice that
+                // the largest p is 1 / total, and every p is off by at most (EPL + 27) u of it: 3 u for its exponent (1.6 |t| 2^t)
+                // and exponential, EPL + 5 for the sum's steps and 17 for its terms (1.6 times the mean |t|, at most 10, and
+                // 2), 2 for the division and the product; the difference of two by twice that
                 tol = 0x1p-17f * inv;
             }
             if (biased) {  // (from the L1: the same for every row)

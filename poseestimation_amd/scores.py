@@ -12,8 +12,9 @@ with a row of scores per question instead (over coordinate bins, classes or toke
 Scores are torch tensors on a GPU, ``(rows, columns)`` in float32, bfloat16 or float16; rows may be any
 distance apart (a slice of a padded buffer, an expanded row), columns are next to each other.  Calls are
 queued on the current stream of the tensors' device and do not wait; they can be captured into a graph.
-The functions take no part in autograd: a training step calls the backward form itself.  Bad arguments
-raise ``ValueError``.  Nothing here has a counterpart in the reference.
+A row's result depends on that row alone, not on its place or the other rows of the call; calls of other
+shapes may add in another order.  The functions take no part in autograd: a training step calls the backward
+form itself.  Bad arguments raise ``ValueError``.  Nothing here has a counterpart in the reference.
 """
 from collections import namedtuple
 
@@ -145,7 +146,8 @@ def token_logprobs(logits, tokens=None, top=0, widths=None):
 def token_logprobs_backward(logits, stats, tokens=None, grad_logp=None, grad_entropy=None, widths=None, out=None):
     """The gradient with respect to the logits, of their type, from that of ``logp`` (shaped like ``tokens``) and of
     ``entropy``; ``stats`` is the forward call's.  The alternatives' log probabilities are differentiated by passing
-    ``top_index`` as tokens.  Tokens that are not given contribute nothing, a token named twice counts twice;
+    ``top_index`` as tokens.  Tokens that are not given contribute nothing, one that the row does not hold what a
+    masked logit would (-p_j g at every column), a token named twice counts twice;
     columns behind a row's width and rows with nothing above -inf get 0.  ``out``: where to put it; the logits
     themselves are allowed."""
     code, rows, columns, stride = _rows(logits, 'logits')
@@ -211,7 +213,7 @@ def route_experts(logits, top, score='softmax', bias=None, groups=1, top_groups=
     weights = torch.empty((rows, top), dtype=torch.float32, device=dev)
     index = torch.empty((rows, top), dtype=torch.int32, device=dev)
     rc = _ffi.lib().pd_route_experts(logits.data_ptr(), code, rows, experts, stride, _address(bias), score, groups, top_groups,
-                                     group_score, top, 1 if renormalise else 0, scale, weights.data_ptr(), index.data_ptr(),
+                                     group_score, top, 1 if renormalise else 0, float(scale), weights.data_ptr(), index.data_ptr(),
                                      _stream(dev))
     if rc:
         _raise(rc)
@@ -235,7 +237,7 @@ def route_experts_backward(logits, index, grad_weights, score='softmax', renorma
     grad_weights = _like(grad_weights, 'grad_weights', torch.float32, ((rows, top),), dev)
     out, out_stride = _grad_out(out, logits)
     rc = _ffi.lib().pd_route_experts_grad(logits.data_ptr(), code, rows, experts, stride, index.data_ptr(), grad_weights.data_ptr(),
-                                          score, top, 1 if renormalise else 0, scale, out.data_ptr(), out_stride, _stream(dev))
+                                          score, top, 1 if renormalise else 0, float(scale), out.data_ptr(), out_stride, _stream(dev))
     if rc:
         _raise(rc)
     return out

@@ -55,7 +55,7 @@ def _close(got, want, tol, what):
     inf = np.isinf(want)
     assert np.array_equal(got[inf], want[inf]) and np.array_equal(np.isinf(got), inf), what
     fine = np.isfinite(want)
-    off = np.abs(got - want)[fine] - np.broadcast_to(tol, want.shape)[fine]
+    off = np.abs(got[fine] - want[fine]) - np.broadcast_to(tol, want.shape)[fine]
     assert not off.size or off.max() <= 0, '%s: %g over its tolerance' % (what, off.max())
 
 
@@ -148,7 +148,9 @@ def test_logprobs_of_masked_infinite_equal_and_nan_rows(cols, dtype):
     x[13, cols // 3] = high
     x[14] = (torch.arange(cols, device='cuda') % 4).to(x.dtype)                          # four values, many ties
     top = min(cols, 40)
-    _check_many(x, _tokens(15, cols, 4, seed=cols), top)
+    # (thousands of rows: several to a wavefront where they are short)
+    _check_many(x, _tokens(15, cols, 4, seed=cols), top, times=1200 if cols < 1000 else 19)
+    _check_many(x, _tokens(15, cols, 20, seed=cols), min(5, cols), times=1200 if cols < 1000 else 300 if cols < 5000 else 19)
     _check_logprobs(x[:1], None, 0)
 
 
@@ -163,6 +165,23 @@ def test_alternatives_that_all_lie_in_few_lanes(cols, period):
     for top in (3, 64):
         _check_many(x, None, top, times=128)
     _check_many(x.bfloat16(), None, 50, times=128)
+
+
+@pytest.mark.parametrize('dtype', ['f32', 'bf16'])
+def test_alternatives_of_short_rows_that_lie_in_few_lanes_and_of_many(dtype):
+    """Columns as they are dealt out to 16, 32 or 64 lanes in pieces of 4 or 8: all the large ones to one lane."""
+    piece = 4 if dtype == 'f32' else 8
+    for cols, lanes in ((500, 16), (1000, 32), (2000, 64), (500, 64)):
+        x = _rows(4, cols, dtype, seed=cols)
+        column = torch.arange(cols, device='cuda')
+        for r, lane in enumerate((3, 0, lanes - 1, 7)):
+            mine = (column // piece) % lanes == lane
+            x[r] = torch.where(mine, 20 + (column if r % 2 else -column).float() / 32, x[r].float()).to(x.dtype)
+        for top in (1, 5, 8, 13, 30):
+            _check_many(x, None, top, times=64 * 4096 // lanes // 4)
+    for rows, cols in ((5, 300), (3, 1000), (2, 2000), (4, 100), (3, 3000)):
+        for top in (17, 20, 33, 50, 64):
+            _check_logprobs(_rows(rows, cols, dtype, seed=top), None, top)
 
 
 @pytest.mark.parametrize('cols, top', [(131072, 64), (600000, 20), (1500000, 64)])

@@ -79,6 +79,16 @@ def test_no_rows_are_no_work(call):
     assert call(rows=0, x=None) == _ffi.PD_OK
 
 
+def test_a_workspace_is_needed_for_few_long_rows_only():
+    need = _ffi.lib().pd_token_logprobs_workspace
+    assert need(_ffi.F32, 4, 2048, 64) == need(_ffi.BF16, 4096, 131072, 5) == need(_ffi.F16, 100, 131072, 5) == 0
+    assert need(_ffi.F32, 0, 1 << 20, 5) == need(_ffi.F32, 4, (1 << 24) + 1, 5) == need(9, 4, 1 << 20, 5) == 0
+    for rows, cols, top in ((1, 131072, 0), (1, 1 << 24, 64), (32, 131072, 5), (1000, 200000, 3)):
+        bytes_ = need(_ffi.BF16, rows, cols, top)
+        # between two and 256 slices of a row, 12 bytes of statistics and `top` keys of 8 each
+        assert 2 * rows * (12 + 8 * top) <= bytes_ <= 256 * rows * (12 + 8 * top) + 16
+
+
 def test_python_functions_refuse_what_is_not_on_a_gpu_or_misshapen():
     x = torch.zeros(4, 16)
     for fn in (lambda v: scores.token_logprobs(v, top=1), lambda v: scores.route_experts(v, 2),
