@@ -123,6 +123,7 @@ __device__ __forceinline__ uint32_t sc_key_place(uint64_t k) { return ~(uint32_t
 
 struct SumOp { template <typename T> __device__ T operator()(T a, T b) const { return a + b; } };
 struct MaxOp { template <typename T> __device__ T operator()(T a, T b) const { return a > b ? a : b; } };
+struct DMaxOp { __device__ double operator()(double a, double b) const { return fmax(a, b); } };
 struct FMaxOp { __device__ float operator()(float a, float b) const { return fmaxf(a, b); } };
 struct MinOp { template <typename T> __device__ T operator()(T a, T b) const { return a < b ? a : b; } };
 
@@ -1072,38 +1073,44 @@ __device__ __forceinline__ void sc_route_put(const RouteArgs& a, int64_t r, int 
 __device__ __forceinline__ void sc_route_row(const RouteArgs& a, int64_t r, int lane, double* by) {
     const int E = a.experts;
     const int64_t row = r * a.stride;
+    // (a lane's experts are lane, lane + 64, ..: nobody else's until the groups look at them; four loads in flight)
+#pragma unroll 4
+    for (int j = lane; j < E; j += 64) by[j] = sc_logit(a.x, a.dtype, row + j);
     double m = 0, total = 0;
     if (!a.sigmoid) {
-        float big = -INFINITY;
+        double big = -INFINITY;
 #pragma nounroll
-        for (int j = lane; j < E; j += 64) big = fmaxf(big, sc_logit(a.x, a.dtype, row + j));
-        big = sc_wave(big, FMaxOp());
+        for (int j = lane; j < E; j += 64) big = fmax(big, by[j]);
+        big = sc_wave(big, DMaxOp());
         if (big > -INFINITY) {
             m = big;
 #pragma nounroll
-            for (int j = lane; j < E; j += 64) total += exp(sc_logit(a.x, a.dtype, row + j) - m);
+            for (int j = lane; j < E; j += 64) total += exp(by[j] - m);
         }
         total = sc_wave(total, SumOp());
     }
     const bool by_p = a.bias || (a.groups > 1 && a.top2);  // else by the logits alone
+    if (by_p)
 #pragma nounroll
-    for (int j = lane; j < E; j += 64) {
-        const double x = sc_logit(a.x, a.dtype, row + j);
-        double v = x;
-        if (by_p) v = a.sigmoid ? 1 / (1 + exp(-x)) : total > 0 ? exp(x - m) / total : 0.0;
-        if (a.bias) v += a.bias[j];
-        by[j] = v >= -1e300 ? v : -1e300;  // -inf and NaN behind all others
-    }
+        for (int j = lane; j < E; j += 64)
+            by[j] = a.sigmoid ? 1 / (1 + exp(-by[j])) : total > 0 ? exp(by[j] - m) / total : 0.0;
+    if (a.bias)
+#pragma unroll 4
+        for (int j = lane; j < E; j += 64) by[j] += a.bias[j];
+#pragma nounroll
+    for (int j = lane; j < E; j += 64) by[j] = by[j] >= -1e300 ? by[j] : -1e300;  // -inf and NaN behind all others
     pd_wave_sync();
     uint64_t kept = ~0ull;
     if (a.groups > 1) {
         double mine = -INFINITY;  // lane g: group g's
         if (lane < a.groups) {
             double b1 = -INFINITY, b2 = -INFINITY;
-#pragma nounroll
-            for (int j = lane * a.per_group; j < (lane + 1) * a.per_group; ++j) {
-                b2 = fmax(b2, fmin(b1, by[j]));
-                b1 = fmax(b1, by[j]);
+            const double* of = by + lane * a.per_group;
+#pragma unroll 8
+            for (int j = 0; j < a.per_group; ++j) {
+                const double v = of[j];
+                b2 = fmax(b2, fmin(b1, v));
+                b1 = fmax(b1, v);
             }
             mine = a.top2 && a.per_group > 1 ? b1 + b2 : b1;
         }
@@ -1125,10 +1132,13 @@ __device__ __forceinline__ void sc_route_row(const RouteArgs& a, int64_t r, int 
     for (int k = 0; k < a.top; ++k) {
         double best = -INFINITY;
         int at = E;
-#pragma nounroll
-        for (int j = lane; j < E; j += 64)
-            if (by[j] > best) best = by[j], at = j;
-        const double top = sc_wave(best, MaxOp());
+#pragma unroll 4
+        for (int j = lane; j < E; j += 64) {
+            const double v = by[j];
+            at = v > best ? j : at;
+            best = fmax(best, v);
+        }
+        const double top = sc_wave(best, DMaxOp());
         at = (int)sc_wave((uint32_t)(best == top ? at : E), MinOp());
         if ((at & 63) == lane && at < E) by[at] = -INFINITY;
         if (lane == k) chosen = at;
