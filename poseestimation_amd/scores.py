@@ -45,6 +45,8 @@ def _rows(x, name):
 
 def _like(x, name, dtype, shapes, device):
     """``x`` as a contiguous tensor of ``dtype`` with one of the shapes, on the device."""
+    if isinstance(x, torch.Tensor) and x.dtype is dtype and x.shape == shapes[0] and x.device == device and x.is_contiguous():
+        return x
     if not isinstance(x, torch.Tensor) or tuple(x.shape) not in shapes or x.device != device:
         raise ValueError('%s must be a tensor of shape %s on %s' % (name, ' or '.join(map(str, shapes)), device))
     if x.dtype != dtype:

@@ -597,6 +597,28 @@ def test_refusals_on_the_gpu():
     assert s.route_experts(empty, 3).index.shape == (0, 3) and s.route_experts_backward(empty, idx[:0], g[:0]).shape == (0, 64)
 
 
+def test_calls_for_another_device_than_the_current_one(monkeypatch):
+    """With the device reported as another one first, each function calls itself under the tensors' own: the same answer."""
+    s = _scores()
+    x, tokens = _rows(6, 300, 'bf16'), _tokens(6, 300, 2)
+    widths = torch.tensor([300, 200, 100, 3, 0, 299], dtype=torch.int32, device='cuda')
+    g, ge, bias = torch.randn(6, 2, device='cuda'), torch.randn(6, device='cuda'), torch.randn(300, device='cuda') * 0.01
+    stats = s.token_logprobs(x, tokens, 4, widths).stats
+    index = s.route_experts(x, 2).index
+    out = torch.empty_like(x)
+    how = dict(score='sigmoid', bias=bias, groups=10, top_groups=3, group_score='top2', renormalise=False, scale=1.5)
+    calls = [lambda: s.token_logprobs(x, tokens, 4, widths), lambda: s.route_experts(x, 5, **how),
+             lambda: (s.token_logprobs_backward(x, stats, tokens, g, ge, widths, out).clone(),),
+             lambda: (s.route_experts_backward(x, index, g, 'sigmoid', False, 1.5, out).clone(),)]
+    want = [c() for c in calls]
+    answers = []
+    monkeypatch.setattr(s, '_current', lambda device: answers.pop(0))
+    for call, w in zip(calls, want):
+        answers[:] = [False, True]
+        got = call()
+        assert not answers and all(torch.equal(a, b) for a, b in zip(got, w))
+
+
 def test_calls_on_two_streams_at_once():
     s = _scores()
     xs = [_rows(3, 140001, 'bf16', seed=k) for k in range(4)]
