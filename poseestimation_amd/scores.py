@@ -50,10 +50,11 @@ def _like(x, name, dtype, shapes, device):
     if not isinstance(x, torch.Tensor) or tuple(x.shape) not in shapes or x.device != device:
         raise ValueError('%s must be a tensor of shape %s on %s' % (name, ' or '.join(map(str, shapes)), device))
     if x.dtype != dtype:
-        if x.is_floating_point() != dtype.is_floating_point or x.dtype == torch.bool or x.is_complex():
+        if x.is_floating_point() != dtype.is_floating_point or x.dtype in (torch.bool, torch.uint64) or x.is_complex():
             raise ValueError('%s must hold %s, got %s' % (name, 'numbers' if dtype.is_floating_point else 'whole numbers', x.dtype))
-        # (int32: a larger number stays out of every range)
-        x = x.clamp(-1, 0x7fffffff).to(dtype) if dtype == torch.int32 else x.to(dtype)
+        if dtype == torch.int32 and x.dtype.itemsize >= 4:  # a larger number stays out of every range
+            x = x.to(torch.int64).clamp(-1, 0x7fffffff)
+        x = x.to(dtype)
     return x if x.is_contiguous() else x.contiguous()
 
 

@@ -241,6 +241,22 @@ def test_tokens_given_twice_not_given_and_out_of_the_row():
     _check_logprobs(x, tokens.t().contiguous().t(), 2)
 
 
+@pytest.mark.parametrize('dtype', [torch.uint8, torch.int8, torch.int16, torch.int32, torch.int64])
+def test_tokens_widths_and_indices_of_every_size(dtype):
+    s = _scores()
+    x, tokens = _rows(9, 100, 'bf16'), _tokens(9, 100, 4)
+    widths = torch.arange(9, device='cuda') * 12
+    g = torch.rand(4, 9, device='cuda', dtype=torch.float64).t()
+    want = s.token_logprobs(x, tokens, 3, widths.int())
+    # (columns of the tokens first: copied into the order that is needed)
+    got = s.token_logprobs(x, tokens.t().contiguous().t().to(dtype), 3, widths.to(dtype))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert torch.equal(s.token_logprobs_backward(x, got.stats, tokens.to(dtype), g, widths=widths.to(dtype)),
+                       s.token_logprobs_backward(x, want.stats, tokens, g.float().contiguous(), widths=widths.int()))
+    index = s.route_experts(x, 4).index
+    assert torch.equal(s.route_experts_backward(x, index.to(dtype), g), s.route_experts_backward(x, index, g.float().contiguous()))
+
+
 def test_rows_whose_offsets_pass_32_bits():
     store = torch.empty((1 << 32) + (1 << 20), dtype=torch.bfloat16, device='cuda')
     x = store.as_strided((3, 1000), ((1 << 31) + 8, 1))

@@ -100,6 +100,22 @@ def test_python_functions_refuse_what_is_not_on_a_gpu_or_misshapen():
     assert scores.TokenLogprobs._fields == ('logp', 'entropy', 'top_logp', 'top_index', 'stats')
 
 
+@pytest.mark.parametrize('dtype', [torch.uint8, torch.int8, torch.int16, torch.int32, torch.int64, torch.uint16, torch.uint32])
+def test_whole_numbers_of_every_size_are_taken(dtype):
+    x = torch.tensor([5, 100, 3], dtype=dtype)
+    for to in (torch.int32, torch.int64):
+        got = scores._like(x, 'x', to, ((3,),), x.device)
+        assert got.dtype == to and got.tolist() == [5, 100, 3]
+
+
+def test_whole_numbers_past_32_bits_stay_out_of_range():
+    x = torch.tensor([1 << 32, -(1 << 32) + 2, (1 << 63) - 1])
+    assert scores._like(x, 'x', torch.int32, ((3,),), x.device).tolist() == [0x7fffffff, -1, 0x7fffffff]
+    for dtype in (torch.bool, torch.uint64):
+        with pytest.raises(ValueError):
+            scores._like(x.to(dtype), 'x', torch.int32, ((3,),), x.device)
+
+
 def test_the_restated_gradients_agree_with_differences():
     rng = np.random.default_rng(5)
     h = 1e-5
