@@ -1334,14 +1334,19 @@ __global__ __launch_bounds__(SC_WG) void k_route(RouteArgs a) {
     }
             SC_TOP2_STEP(1) SC_TOP2_STEP(2) SC_TOP2_STEP(4) SC_TOP2_STEP(8) SC_TOP2_STEP(16) SC_TOP2_STEP(32)
 #undef SC_TOP2_STEP
-            const float mine = a.top2 && a.per_group > 1 ? b1 + b2 : b1;
+            const bool two = a.top2 && a.per_group > 1;
+            const float mine = two ? b1 + b2 : b1;
             if constexpr (CLOSE) {
-                const float off = 2 * tol + 0x1p-21f * fabsf(mine);
+                // What the float64 score lies between.  Two p are off by tol together; b1 and b2 are off by a rounding of the
+                // sum with the bias each, whatever is left of them in b1 + b2, that by one, and lo and hi by one: 3 u
+                // (|b1| + |b2|), and 4 u are taken.  A bound past float32 leaves it open.
+                const float off = tol + 0x1p-22f * (fabsf(b1) + (two ? fabsf(b2) : 0.0f));
+                const float lo = off < INFINITY ? mine - off : -INFINITY, hi = off < INFINITY ? mine + off : INFINITY;
                 int above = 0, maybe = 0;
                 for (int k = 0; k < a.groups; ++k) {
-                    const float o = __shfl(mine, first + k * a.group_lanes);
-                    above += o > mine + off;
-                    maybe += k != g && !(o < mine - off);
+                    const float o_lo = __shfl(lo, first + k * a.group_lanes), o_hi = __shfl(hi, first + k * a.group_lanes);
+                    above += o_lo > hi;
+                    maybe += k != g && !(o_hi < lo);
                 }
                 kept = maybe < a.top_groups;
                 again = g < a.groups && !kept && above < a.top_groups;

@@ -1,0 +1,41 @@
+"""Rows of scores on the GPU at their edges: group sums that cancel, biases of NaN and infinities, what results share with
+each other and with autograd, gradients next to their logits, rows that share a wavefront.  Tolerances as in
+``test_gpu_scores``, whose checks these tests use."""
+import math
+
+import numpy as np
+import pytest
+
+from tests import scores_ref as ref
+from tests.test_gpu_scores import TYPES, _check_logprobs, _check_route, _np, _rows, _scores, _tokens
+
+torch = pytest.importorskip('torch')
+pytestmark = pytest.mark.gpu
+
+
+# ---- routing in groups by sums ---------------------------------------------------------------
+
+def _alternating(experts, groups, big):
+    """One expert of every group pushed up by ``big``, all others down: the two largest of a group cancel."""
+    bias = torch.full((experts,), -big, device='cuda')
+    bias[::experts // groups] = big
+    return bias
+
+
+def test_route_by_group_sums_that_cancel():
+    x = torch.tensor([[-0.29003906, 0.11914062, -0.04101562, -0.13085938]], device='cuda')
+    bias = torch.tensor([1e4, -1e4, 1e4, -1e4], device='cuda')
+    how = dict(score='sigmoid', groups=2, top_groups=1, group_score='top2', bias=bias)
+    assert _check_route(x, 2, **how).index[0].tolist() == [0, 1]        # 0.957744 against 0.957079
+
+
+@pytest.mark.parametrize('score', ['softmax', 'sigmoid'])
+@pytest.mark.parametrize('big', [1e2, 1e3, 1e4, 1e5])
+def test_route_by_group_sums_next_to_large_biases(big, score):
+    for experts, groups, top_groups in ((64, 8, 4), (128, 4, 1), (48, 16, 5)):
+        bias = _alternating(experts, groups, big)
+        for k, scale in enumerate((1e-3, 0.05, 1.0)):    # p + p of two groups apart by less and by more than a step of `big`
+            gen = torch.Generator().manual_seed(k)
+            x = (torch.randn(150, experts, generator=gen) * scale).cuda()
+            for b in (bias, -bias, bias + torch.randn(experts, generator=gen).cuda()):
+                _check_route(x, 4, bias=b, score=score, groups=groups, top_groups=top_groups, group_score='top2')
