@@ -1313,7 +1313,7 @@ __global__ __launch_bounds__(SC_WG) void k_route(RouteArgs a) {
                 float b[EPL];
                 sc_route_read<F32, EPL>(a.bias, place, have, full, b);
 #pragma unroll
-                for (int j = 0; j < EPL; ++j) s[j] += b[j];
+                for (int j = 0; j < EPL; ++j) s[j] = fmaxf(s[j] + b[j], -INFINITY);  // a bias of NaN counts as -inf
             }
         }
         if (a.groups > 1) {

@@ -39,3 +39,20 @@ def test_route_by_group_sums_next_to_large_biases(big, score):
             x = (torch.randn(150, experts, generator=gen) * scale).cuda()
             for b in (bias, -bias, bias + torch.randn(experts, generator=gen).cuda()):
                 _check_route(x, 4, bias=b, score=score, groups=groups, top_groups=top_groups, group_score='top2')
+
+
+@pytest.mark.parametrize('score', ['softmax', 'sigmoid'])
+def test_route_by_group_sums_with_nan_biases(score):
+    """An expert whose bias is NaN comes behind all others, and adds nothing to its group."""
+    logit = torch.tensor([0.9, 0.5, 0.1, 0.6, 0.7, 0.2], device='cuda').logit()
+    x = logit[None].expand(3, 6)
+    bias = torch.tensor([0, math.nan, 0, 0, 0, 0], device='cuda')
+    how = dict(score=score, groups=2, top_groups=1, group_score='top2')
+    _check_route(x, 2, bias=bias, **how)             # sigmoid: 0.9 + 0.1 against 0.6 + 0.7
+    gen = torch.Generator().manual_seed(2)
+    for experts, groups, top_groups, top in ((64, 8, 4, 8), (256, 8, 2, 6), (24, 3, 1, 2), (512, 32, 5, 16)):
+        bias = torch.randn(experts, generator=gen) * 0.05
+        bias.view(groups, -1)[:, ::3] = math.nan     # (two or more are left in every group)
+        x = _rows(70, experts, 'f32', seed=experts, scale=1.0)
+        for group_score in ('top2', 'max'):
+            _check_route(x, top, bias=bias.cuda(), score=score, groups=groups, top_groups=top_groups, group_score=group_score)
