@@ -456,7 +456,8 @@ int pd_token_logprobs_grad(const void* logits, int dtype, int64_t rows, int64_t 
  * top_groups best groups are chosen first, by their largest value (PD_GROUP_MAX) or the sum of their two
  * largest of p, or p + bias (PD_GROUP_TOP2); only their experts are eligible.
  *   weights[r][i] = scale * p_i, with renormalise scale * p_i / (sum of the chosen p); index[r][i] the expert.
- * A logit of -inf has p = 0; a bias of -inf (or NaN) puts an expert behind all others.  Rows with nothing
+ * A logit of -inf has p = 0; a bias of -inf (or NaN) puts an expert behind all others: a group with fewer than
+ * two others has a sum of -inf, all such groups alike; one with a bias of +inf counts as +inf.  Rows with nothing
  * above -inf get weights of 0 under softmax and, where the sum is 0, when renormalised.  A row that holds a
  * NaN (softmax: or +inf): weights NaN, index -1. */
 enum { PD_SCORE_SOFTMAX = 0, PD_SCORE_SIGMOID = 1 };

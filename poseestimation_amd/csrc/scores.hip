@@ -1112,7 +1112,9 @@ __device__ __forceinline__ void sc_route_row(const RouteArgs& a, int64_t r, int 
                 b2 = fmax(b2, fmin(b1, v));
                 b1 = fmax(b1, v);
             }
-            mine = a.top2 && a.per_group > 1 ? b1 + b2 : b1;
+            mine = b1;
+            // (-1e300 stands for -inf, which a sum of finite ones never is; one of +inf and -inf counts as +inf)
+            if (a.top2 && a.per_group > 1) mine = b2 > -1e300 || b1 == INFINITY ? b1 + b2 : -INFINITY;
         }
         int rank = 0;
 #pragma nounroll
@@ -1339,9 +1341,10 @@ __global__ __launch_bounds__(SC_WG) void k_route(RouteArgs a) {
             if constexpr (CLOSE) {
                 // What the float64 score lies between.  Two p are off by tol together; b1 and b2 are off by a rounding of the
                 // sum with the bias each, whatever is left of them in b1 + b2, that by one, and lo and hi by one: 3 u
-                // (|b1| + |b2|), and 4 u are taken.  A bound past float32 leaves it open.
+                // (|b1| + |b2|), and 4 u are taken.  A bound past float32 leaves it open.  A term of -inf is that exactly.
                 const float off = tol + 0x1p-22f * (fabsf(b1) + (two ? fabsf(b2) : 0.0f));
-                const float lo = off < INFINITY ? mine - off : -INFINITY, hi = off < INFINITY ? mine + off : INFINITY;
+                const bool out = (two ? b2 : b1) == -INFINITY && b1 < INFINITY;
+                const float lo = !out && off < INFINITY ? mine - off : -INFINITY, hi = off < INFINITY ? mine + off : out ? -INFINITY : INFINITY;
                 int above = 0, maybe = 0;
                 for (int k = 0; k < a.groups; ++k) {
                     const float o_lo = __shfl(lo, first + k * a.group_lanes), o_hi = __shfl(hi, first + k * a.group_lanes);

@@ -198,8 +198,9 @@ def route_experts(logits, top, score='softmax', bias=None, groups=1, top_groups=
     (``'top2'``, of p or p + bias).  ``Routes(weights, index)``, both (rows, top) in descending order: weights are
     ``scale`` * p, with ``renormalise`` divided by the sum of the chosen p.
 
-    A bias of -inf puts an expert behind all others.  A row whose chosen p sum to 0 gets weights of 0 when
-    renormalised.  A row that holds a NaN (softmax: or +inf): weights NaN, index -1."""
+    A bias of -inf or NaN puts an expert behind all others; a group with fewer than two others has a sum of -inf, all
+    such groups alike (the lower index first), and one with a bias of +inf counts as +inf.  A row whose chosen p sum to 0
+    gets weights of 0 when renormalised.  A row that holds a NaN (softmax: or +inf): weights NaN, index -1."""
     code, rows, experts, stride = _rows(logits, 'logits')
     dev = logits.device
     if not _current(dev):

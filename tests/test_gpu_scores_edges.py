@@ -56,3 +56,36 @@ def test_route_by_group_sums_with_nan_biases(score):
         x = _rows(70, experts, 'f32', seed=experts, scale=1.0)
         for group_score in ('top2', 'max'):
             _check_route(x, top, bias=bias.cuda(), score=score, groups=groups, top_groups=top_groups, group_score=group_score)
+
+
+@pytest.mark.parametrize('score', ['softmax', 'sigmoid'])
+def test_route_by_group_sums_with_experts_shut_out(score):
+    """A group with fewer than two experts that are not shut out has a sum of -inf, all such groups alike."""
+    gen = torch.Generator().manual_seed(3)
+    for experts, groups, top_groups, top in ((64, 8, 4, 8), (16, 4, 1, 2), (256, 8, 2, 6), (60, 20, 7, 5), (8, 8, 3, 3), (1000, 40, 3, 20)):
+        per = experts // groups
+        x = _rows(40, experts, 'f32', seed=groups, scale=1.0)
+        for left in range(per + 1):                  # of group g: g mod (left + 1) experts, so that there are some of every kind
+            if left > 6 and left < per:
+                continue
+            bias = torch.randn(experts, generator=gen) * 0.05
+            for g in range(groups):
+                out = torch.randperm(per, generator=gen)[min(per, (g * 3 + 1) % (left + 1)):]
+                bias[g * per + out] = -math.inf if left % 2 else math.nan
+            for group_score in ('top2', 'max'):
+                _check_route(x, top, bias=bias.cuda(), score=score, groups=groups, top_groups=top_groups, group_score=group_score)
+    x = _rows(9, 64, 'f32')
+    for low in (-math.inf, torch.finfo(torch.float32).min):       # everybody; sums past float32
+        _check_route(x, 5, bias=torch.full((64,), low, device='cuda'), score=score, groups=8, top_groups=3, group_score='top2')
+
+
+@pytest.mark.parametrize('score', ['softmax', 'sigmoid'])
+def test_route_by_group_sums_with_a_bias_of_plus_infinity(score):
+    """A group that holds one comes before all that hold none, also where its other experts are shut out."""
+    x = _rows(30, 64, 'f32', scale=1.0)
+    for other in (0.0, -math.inf):
+        bias = torch.full((64,), other, device='cuda')
+        bias[:48] = 0
+        bias[61] = math.inf
+        r = _scores().route_experts(x, 3, score=score, bias=bias, groups=4, top_groups=1, group_score='top2')
+        assert (r.index[:, 0] == 61).all() and (r.index >= 48).all()
