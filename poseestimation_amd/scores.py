@@ -120,24 +120,19 @@ def token_logprobs(logits, tokens=None, top=0, widths=None):
         n_tok = shape[1] if len(shape) == 2 else 1
     if widths is not None:
         widths = _like(widths, 'widths', torch.int32, ((rows,),), dev)
-    # one allocation for what a call returns, cut into the parts, behind the workspace where that is small
     L = _ffi.lib()
     ws_bytes = L.pd_token_logprobs_workspace(code, rows, columns, top)
-    at = ws_bytes // 4 if ws_bytes <= 1 << 18 else 0
-    store = torch.empty(at + rows * (n_tok + 2 * top + 4), dtype=torch.float32, device=dev)
-    ws = None
-    if ws_bytes:
-        ws = store if at else torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-    entropy = store.as_strided((rows,), (1,), at)
-    stats = store.as_strided((rows, 3), (3, 1), at + rows)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+    # Each result a tensor of its own: one that is kept keeps nothing else, and one that is written marks no other as changed.
+    # (Sizes one by one: 1.25 us an allocation, 1.6 with a tuple.)
     logp = top_logp = top_index = None
-    at += 4 * rows
+    entropy = torch.empty(rows, dtype=torch.float32, device=dev)
+    stats = torch.empty(rows, 3, dtype=torch.float32, device=dev)
     if top:
-        top_logp = store.as_strided((rows, top), (top, 1), at)
-        top_index = store.view(torch.int32).as_strided((rows, top), (top, 1), at + rows * top)
-        at += 2 * rows * top
+        top_logp = torch.empty(rows, top, dtype=torch.float32, device=dev)
+        top_index = torch.empty(rows, top, dtype=torch.int32, device=dev)
     if shape is not None:
-        logp = store.as_strided(shape, (n_tok, 1) if len(shape) == 2 else (1,), at)
+        logp = torch.empty(*shape, dtype=torch.float32, device=dev)
     rc = L.pd_token_logprobs(logits.data_ptr(), code, rows, columns, stride, _address(widths), _address(tokens), n_tok, top,
                              _address(logp), entropy.data_ptr(), stats.data_ptr(), _address(top_logp), _address(top_index),
                              _address(ws), ws_bytes, _stream(dev))

@@ -89,3 +89,22 @@ def test_route_by_group_sums_with_a_bias_of_plus_infinity(score):
         bias[61] = math.inf
         r = _scores().route_experts(x, 3, score=score, bias=bias, groups=4, top_groups=1, group_score='top2')
         assert (r.index[:, 0] == 61).all() and (r.index >= 48).all()
+
+
+# ---- what results share ----------------------------------------------------------------------
+
+@pytest.mark.parametrize('rows, cols', [(5, 300), (3, 5000), (2, 140001)])
+def test_results_are_tensors_of_their_own(rows, cols):
+    s = _scores()
+    x, tokens = _rows(rows, cols, 'bf16'), _tokens(rows, cols, 2)
+    r = s.token_logprobs(x, tokens, top=3)
+    # nothing else is kept alive by one of them, and writing one does not mark the others as changed
+    assert [part.untyped_storage().nbytes() for part in r] == [part.numel() * 4 for part in r]
+    assert [part._is_view() for part in r] == [False] * 5 and all(part.is_contiguous() for part in r)
+    weight = torch.ones(rows, device='cuda', requires_grad=True)
+    loss = (weight * r.entropy).sum()
+    r.logp.mul_(2)
+    r.top_index.fill_(0)
+    r.stats.zero_()
+    loss.backward()
+    assert torch.equal(weight.grad, r.entropy)
