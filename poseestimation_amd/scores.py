@@ -14,7 +14,9 @@ distance apart (a slice of a padded buffer, an expanded row), columns are next t
 queued on the current stream of the tensors' device and do not wait; they can be captured into a graph.
 A row's result depends on that row alone, not on its place or the other rows of the call; calls of other
 shapes may add in another order.  The functions take no part in autograd: a training step calls the backward
-form itself.  Bad arguments raise ``ValueError``.  Nothing here has a counterpart in the reference.
+form itself, and where gradients are recorded the forward ones refuse logits that require one (pass
+``logits.detach()``).  Gradients have no gradient.  Bad arguments raise ``ValueError``.  Nothing here has a counterpart
+in the reference.
 """
 from collections import namedtuple
 
@@ -28,6 +30,13 @@ _GROUP_SCORES = {'max': _ffi.GROUP_MAX, 'top2': _ffi.GROUP_TOP2}
 
 TokenLogprobs = namedtuple('TokenLogprobs', 'logp entropy top_logp top_index stats')
 Routes = namedtuple('Routes', 'weights index')
+
+
+def _no_grad(logits):
+    """Refuses logits whose gradient autograd would lose: what is made of them here carries none."""
+    if isinstance(logits, torch.Tensor) and logits.requires_grad and torch.is_grad_enabled():
+        raise ValueError('the logits require a gradient, which autograd does not get from here: pass logits.detach() '
+                         '(or call under torch.no_grad()) and call the backward form')
 
 
 def _rows(x, name):
@@ -107,6 +116,7 @@ def token_logprobs(logits, tokens=None, top=0, widths=None):
 
     A negative token is not given: 0.  A token that the row does not hold: -inf.  A row with nothing above -inf:
     -inf, entropy 0, alternatives 0, 1, .. .  A row that holds a NaN or +inf: NaN, alternatives -1."""
+    _no_grad(logits)
     code, rows, columns, stride = _rows(logits, 'logits')
     dev = logits.device
     if not _current(dev):
@@ -196,6 +206,7 @@ def route_experts(logits, top, score='softmax', bias=None, groups=1, top_groups=
     A bias of -inf or NaN puts an expert behind all others; a group with fewer than two others has a sum of -inf, all
     such groups alike (the lower index first), and one with a bias of +inf counts as +inf.  A row whose chosen p sum to 0
     gets weights of 0 when renormalised.  A row that holds a NaN (softmax: or +inf): weights NaN, index -1."""
+    _no_grad(logits)
     code, rows, experts, stride = _rows(logits, 'logits')
     dev = logits.device
     if not _current(dev):

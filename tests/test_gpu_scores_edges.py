@@ -108,3 +108,23 @@ def test_results_are_tensors_of_their_own(rows, cols):
     r.stats.zero_()
     loss.backward()
     assert torch.equal(weight.grad, r.entropy)
+
+
+# ---- autograd --------------------------------------------------------------------------------
+
+def test_logits_that_autograd_would_lose_are_refused():
+    s = _scores()
+    x = _rows(4, 64, 'f32').requires_grad_()
+    for call in (lambda: s.token_logprobs(x, top=2), lambda: s.route_experts(x, 2), lambda: s.token_logprobs(x * 1, top=2)):
+        with pytest.raises(ValueError, match='detach'):
+            call()
+        with torch.no_grad():
+            call()
+    r, routes = s.token_logprobs(x.detach(), top=2), s.route_experts(x.detach(), 2, bias=torch.zeros(64, device='cuda', requires_grad=True))
+    ones = torch.ones(4, 2, device='cuda')
+    # the backward forms give the gradient itself, and take the logits as they are
+    x.backward(s.token_logprobs_backward(x, r.stats, r.top_index, ones))
+    x.backward(s.route_experts_backward(x, routes.index, ones, renormalise=False))
+    want = torch.log_softmax(x.double(), 1).gather(1, r.top_index.long()).sum() + torch.softmax(x.double(), 1).gather(1, routes.index.long()).sum()
+    (grad,) = torch.autograd.grad(want, x)
+    assert (x.grad - grad).abs().max() < 1e-5
