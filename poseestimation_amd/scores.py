@@ -104,6 +104,12 @@ def _grad_out(out, logits):
     return out, columns if rows <= 1 else stride
 
 
+def _written(out):
+    """The kernels write to an address: tells autograd, which may have kept the tensor for a backward pass."""
+    torch.autograd.graph.increment_version(out)
+    return out
+
+
 def token_logprobs(logits, tokens=None, top=0, widths=None):
     """Log probabilities of the given ``tokens`` (``(rows,)`` or ``(rows, n)``, n <= 64) under the softmax of
     every row, the row's entropy, and its ``top`` (<= 64) largest entries.
@@ -177,13 +183,14 @@ def token_logprobs_backward(logits, stats, tokens=None, grad_logp=None, grad_ent
         grad_entropy = _like(grad_entropy, 'grad_entropy', torch.float32, ((rows,),), dev)
     if widths is not None:
         widths = _like(widths, 'widths', torch.int32, ((rows,),), dev)
+    given = out is not None
     out, out_stride = _grad_out(out, logits)
     rc = _ffi.lib().pd_token_logprobs_grad(logits.data_ptr(), code, rows, columns, stride, _address(widths), stats.data_ptr(),
                                            _address(tokens), n_tok, _address(grad_logp), _address(grad_entropy), out.data_ptr(),
                                            out_stride, _stream(dev))
     if rc:
         _raise(rc)
-    return out
+    return _written(out) if given else out
 
 
 def _score_code(table, value, name):
@@ -245,9 +252,10 @@ def route_experts_backward(logits, index, grad_weights, score='softmax', renorma
     top = index.shape[1]
     index = _like(index, 'index', torch.int32, ((rows, top),), dev)
     grad_weights = _like(grad_weights, 'grad_weights', torch.float32, ((rows, top),), dev)
+    given = out is not None
     out, out_stride = _grad_out(out, logits)
     rc = _ffi.lib().pd_route_experts_grad(logits.data_ptr(), code, rows, experts, stride, index.data_ptr(), grad_weights.data_ptr(),
                                           score, top, 1 if renormalise else 0, float(scale), out.data_ptr(), out_stride, _stream(dev))
     if rc:
         _raise(rc)
-    return out
+    return _written(out) if given else out

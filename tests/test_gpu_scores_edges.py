@@ -128,3 +128,21 @@ def test_logits_that_autograd_would_lose_are_refused():
     want = torch.log_softmax(x.double(), 1).gather(1, r.top_index.long()).sum() + torch.softmax(x.double(), 1).gather(1, routes.index.long()).sum()
     (grad,) = torch.autograd.grad(want, x)
     assert (x.grad - grad).abs().max() < 1e-5
+
+
+def test_a_gradient_written_over_the_logits_is_seen_by_autograd():
+    s = _scores()
+    for backward in ('logprobs', 'route'):
+        leaf = torch.randn(4, 64, device='cuda', requires_grad=True)
+        logits = leaf.tanh()                          # keeps what it returned for its own backward pass
+        x = logits.detach()
+        r, index = s.token_logprobs(x, top=2), s.route_experts(x, 2).index
+        ones, before = torch.ones(4, 2, device='cuda'), x._version
+        if backward == 'logprobs':
+            s.token_logprobs_backward(x, r.stats, r.top_index, ones, out=x)
+        else:
+            s.route_experts_backward(x, index, ones, out=x)
+        after = x._version
+        assert after == before + 1
+        with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+            logits.sum().backward()
