@@ -1611,14 +1611,40 @@ static int sc_check_rows(const char* fn, const void* x, int dtype, int64_t rows,
     return 0;
 }
 
+// Whether one of `rows` intervals of `width` bytes from x on, x_step apart, meets one of as many from g on, g_step >= width
+// apart.  Mostly told without the rows: by the whole ranges, or where the g lie in the gaps of every multiple of the steps' common
+// divisor (columns next to each other, every other row); with equal steps that decides it.
+static bool sc_rows_meet(uintptr_t x, int64_t x_step, uintptr_t g, int64_t g_step, int64_t rows, int64_t width) {
+    const int64_t to_g = (int64_t)(g - x), x_end = (rows - 1) * x_step + width;  // from x on
+    if (to_g >= x_end || to_g + (rows - 1) * g_step + width <= 0) return false;
+    int64_t step = g_step;
+    for (int64_t b = x_step; b; ) {
+        const int64_t c = step % b;
+        step = b;
+        b = c;
+    }
+    const int64_t at = (to_g % step + step) % step;
+    if (at >= width && at + width <= step) return false;
+    if (x_step == g_step) return true;
+    for (int64_t r = 0; r < rows; ++r) {
+        const int64_t from = to_g + r * g_step;
+        if (from >= x_end) break;
+        if (from + width <= 0) continue;
+        // the first x that ends behind `from`
+        const int64_t k = from < width ? 0 : x_step ? (from - width) / x_step + 1 : rows;
+        if (k < rows && k * x_step < from + width) return true;
+    }
+    return false;
+}
+
 // The gradient's rows: in the logits' own place, or clear of them.
 static int sc_check_grad(const char* fn, const void* x, int dtype, int64_t rows, int64_t cols, int64_t stride, const void* grad,
                          int64_t grad_stride) {
-    if ((uintptr_t)grad % sc_size(dtype)) return sc_fail(fn, "grad is not aligned to its type");
+    const int64_t size = sc_size(dtype);
+    if ((uintptr_t)grad % size) return sc_fail(fn, "grad is not aligned to its type");
     if (grad_stride < cols || grad_stride > INT64_MAX / 8 / rows) return sc_fail(fn, "the rows of grad overlap");
-    const uintptr_t x0 = (uintptr_t)x, x1 = x0 + ((rows - 1) * stride + cols) * sc_size(dtype);
-    const uintptr_t g0 = (uintptr_t)grad, g1 = g0 + ((rows - 1) * grad_stride + cols) * sc_size(dtype);
-    if (g0 < x1 && x0 < g1 && !(g0 == x0 && (grad_stride == stride || rows == 1)))
+    if (grad == x && (grad_stride == stride || rows == 1)) return PD_OK;
+    if (sc_rows_meet((uintptr_t)x, stride * size, (uintptr_t)grad, grad_stride * size, rows, cols * size))
         return sc_fail(fn, "grad overlaps the logits without being them");
     return PD_OK;
 }

@@ -146,3 +146,32 @@ def test_a_gradient_written_over_the_logits_is_seen_by_autograd():
         assert after == before + 1
         with pytest.raises(RuntimeError, match='modified by an inplace operation'):
             logits.sum().backward()
+
+
+# ---- gradients next to their logits ----------------------------------------------------------
+
+def test_gradients_between_the_rows_of_their_logits():
+    """In the columns next to them, in every other row, before and behind them in the same buffer, rows at other distances."""
+    s = _scores()
+    ones = torch.ones(5, 2, device='cuda')
+    for dtype in TYPES.values():
+        def buffer():
+            return _rows(24, 96, 'f32', seed=7).to(dtype)
+        places = [lambda b: (b[:5, :32], b[:5, 32:64]), lambda b: (b[:5, 64:], b[:5, :64]), lambda b: (b[1:10:2], b[:10:2]),
+                  lambda b: (b[:10:2], b[1:11:2]), lambda b: (b[:10:2, :48], b[:5, 48:]), lambda b: (b[:5, 48:], b[:10:2, :48]),
+                  lambda b: (b[:5], b[5:10]), lambda b: (b[2:3, :40].expand(5, 40), b[:5, 40:80]),
+                  lambda b: (b.as_strided((5, 30), (50, 1)), b.as_strided((5, 20), (100, 1), 30)),
+                  lambda b: (b.as_strided((5, 20), (50, 1)), b.as_strided((5, 20), (101, 1), 20)),
+                  lambda b: (b.as_strided((5, 30), (7, 1), 120), b.as_strided((5, 30), (96, 1), 83))]
+        for k, place in enumerate(places):
+            b = buffer()
+            x, out = place(b)
+            out = out[:, :x.shape[1]]
+            x = x[:, :out.shape[1]]
+            plain = x.contiguous()
+            r, index = s.token_logprobs(plain, top=2), s.route_experts(plain, 2).index
+            for want, call in ((s.token_logprobs_backward(plain, r.stats, r.top_index, ones),
+                                lambda: s.token_logprobs_backward(x, r.stats, r.top_index, ones, out=out)),
+                               (s.route_experts_backward(plain, index, ones, renormalise=False),
+                                lambda: s.route_experts_backward(x, index, ones, renormalise=False, out=out))):
+                assert call() is out and torch.equal(out, want) and torch.equal(x, plain), (dtype, k)
