@@ -468,7 +468,9 @@ int pd_route_experts(const void* logits, int dtype, int64_t rows, int64_t expert
 
 /* The gradient of the weights with respect to the logits (the choice itself has none), of their type, every
  * expert of every row.  index: as returned, [rows][top]; entries outside 0..experts-1 are skipped, an expert
- * named twice counts twice.  grad may be the logits themselves (same stride) or must not overlap them. */
+ * named twice counts twice.  So a row that has no order, its index -1, gets 0 where only the chosen logits are
+ * read and NaN where the weights are a softmax that is not renormalised.  grad may be the logits themselves
+ * (same stride) or must not overlap them. */
 int pd_route_experts_grad(const void* logits, int dtype, int64_t rows, int64_t experts, int64_t row_stride,
                           const int32_t* index, const float* grad_weights, int score, int top, int renormalise,
                           float scale, void* grad, int64_t grad_stride, void* stream);

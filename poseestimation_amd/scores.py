@@ -240,7 +240,8 @@ def route_experts(logits, top, score='softmax', bias=None, groups=1, top_groups=
 def route_experts_backward(logits, index, grad_weights, score='softmax', renormalise=True, scale=1.0, out=None):
     """The gradient of ``weights`` with respect to the logits, of their type; ``index`` is the forward call's, the choice
     itself (bias, groups) has no gradient.  Entries of ``index`` that name no expert are skipped, an expert named twice
-    counts twice.  ``out``: where to put it; the logits themselves are allowed."""
+    counts twice.  So a row without an order (its index is -1) gets 0, but NaN where the weights are a softmax that is not
+    renormalised, the one form that reads all of the row.  ``out``: where to put it; the logits themselves are allowed."""
     code, rows, experts, stride = _rows(logits, 'logits')
     dev = logits.device
     if not _current(dev):

@@ -175,3 +175,20 @@ def test_gradients_between_the_rows_of_their_logits():
                                (s.route_experts_backward(plain, index, ones, renormalise=False),
                                 lambda: s.route_experts_backward(x, index, ones, renormalise=False, out=out))):
                 assert call() is out and torch.equal(out, want) and torch.equal(x, plain), (dtype, k)
+
+
+def test_the_routing_gradient_of_rows_without_an_order():
+    """Index -1 names no expert: 0 where only chosen logits are read, NaN where a softmax that is not renormalised reads all."""
+    s = _scores()
+    x = _rows(3, 40, 'f32')
+    x[1, 7] = math.nan
+    g = torch.ones(3, 4, device='cuda')
+    for how in (dict(), dict(score='sigmoid'), dict(score='sigmoid', renormalise=False), dict(renormalise=False)):
+        routes = s.route_experts(x, 4, **how)
+        assert torch.isnan(routes.weights[1]).all() and (routes.index[1] == -1).all()
+        grad = s.route_experts_backward(x, routes.index, g, **how)
+        if how == dict(renormalise=False):
+            assert torch.isnan(grad[1]).all()
+        else:
+            assert not grad[1].any()
+        assert torch.isfinite(grad[[0, 2]]).all()
