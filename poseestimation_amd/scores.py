@@ -204,7 +204,8 @@ def route_experts(logits, top, score='softmax', bias=None, groups=1, top_groups=
     """The ``top`` (<= 32) of the experts (columns, <= 1024) that each row goes to, and their weights.
 
     p is the softmax of the row, or 1 / (1 + exp(-x)) with ``score='sigmoid'``.  Experts are ordered by p + ``bias``
-    (experts,), without bias by the logits, equal ones by the lower index; the order is that of float64 arithmetic.
+    (experts,), without bias by the logits, equal ones by the lower index; the order is that of float64 arithmetic on the
+    logits and on the bias in float32, which one of another type is rounded to.
     With ``groups`` > 1 (<= 64, equal parts of consecutive experts) only the experts of the ``top_groups`` best groups are
     eligible, a group counting by its largest value (``group_score='max'``) or by the sum of its two largest
     (``'top2'``, of p or p + bias).  ``Routes(weights, index)``, both (rows, top) in descending order: weights are

@@ -192,3 +192,12 @@ def test_the_routing_gradient_of_rows_without_an_order():
         else:
             assert not grad[1].any()
         assert torch.isfinite(grad[[0, 2]]).all()
+
+
+def test_a_bias_of_another_type_is_rounded_to_float32_first():
+    s = _scores()
+    x = _rows(20, 64, 'f32')
+    bias = torch.randn(64, dtype=torch.float64, generator=torch.Generator().manual_seed(4)).cuda()
+    for b in (bias, bias.bfloat16(), bias.half()):
+        got, want = s.route_experts(x, 6, bias=b), s.route_experts(x, 6, bias=b.float())
+        assert torch.equal(got.index, want.index) and torch.equal(got.weights, want.weights)
