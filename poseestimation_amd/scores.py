@@ -79,9 +79,13 @@ def _current(device):
     return torch.cuda.current_device() == device.index
 
 
+# The current stream's address itself: making a Stream object of it takes longer than the checks of a small call.  Not a public
+# name of torch, so that it need not be there.
+_raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None)
+
+
 def _stream(device):
-    # (the stream's address itself: making a Stream object of it takes longer than the checks of a small call)
-    return torch._C._cuda_getCurrentRawStream(device.index)
+    return torch.cuda.current_stream(device).cuda_stream if _raw_stream is None else _raw_stream(device.index)
 
 
 def _raise(rc):

@@ -201,3 +201,18 @@ def test_a_bias_of_another_type_is_rounded_to_float32_first():
     for b in (bias, bias.bfloat16(), bias.half()):
         got, want = s.route_experts(x, 6, bias=b), s.route_experts(x, 6, bias=b.float())
         assert torch.equal(got.index, want.index) and torch.equal(got.weights, want.weights)
+
+
+def test_the_stream_is_found_without_torchs_inner_function(monkeypatch):
+    s = _scores()
+    x = _rows(3, 300, 'f32')
+    want = s.token_logprobs(x, top=4)
+    stream = torch.cuda.Stream()
+    assert s._stream(x.device) == torch.cuda.current_stream().cuda_stream
+    monkeypatch.setattr(s, '_raw_stream', None)
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        assert s._stream(x.device) == stream.cuda_stream
+        got = s.token_logprobs(x, top=4)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got[1:], want[1:]))
