@@ -1069,7 +1069,8 @@ __device__ __forceinline__ void sc_route_put(const RouteArgs& a, int64_t r, int 
     }
 }
 
-// A row by one wavefront in float64; by: PD_MAX_EXPERTS values of the wavefront's own.
+// A row by one wavefront in float64, where p + bias or the groups' sums of p order the experts (ROUTE_CLOSE); by: PD_MAX_EXPERTS
+// values of the wavefront's own.
 __device__ __forceinline__ void sc_route_row(const RouteArgs& a, int64_t r, int lane, double* by) {
     const int E = a.experts;
     const int64_t row = r * a.stride;
@@ -1089,8 +1090,6 @@ __device__ __forceinline__ void sc_route_row(const RouteArgs& a, int64_t r, int 
         }
         total = sc_wave(total, SumOp());
     }
-    const bool by_p = a.bias || (a.groups > 1 && a.top2);  // else by the logits alone
-    if (by_p)
 #pragma nounroll
         for (int j = lane; j < E; j += 64)
             by[j] = a.sigmoid ? 1 / (1 + exp(-by[j])) : total > 0 ? exp(by[j] - m) / total : 0.0;
@@ -1126,7 +1125,7 @@ __device__ __forceinline__ void sc_route_row(const RouteArgs& a, int64_t r, int 
     }
 #pragma nounroll
     for (int j = lane; j < E; j += 64) {
-        if (by_p && !a.bias) by[j] = fmax((double)sc_logit(a.x, a.dtype, row + j), -1e300);  // p counted for the groups only
+        if (!a.bias) by[j] = fmax((double)sc_logit(a.x, a.dtype, row + j), -1e300);  // p counted for the groups only
         if (!(kept >> (j / a.per_group) & 1)) by[j] = -INFINITY;
     }
     int chosen = -1;
