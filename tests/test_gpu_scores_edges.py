@@ -216,3 +216,60 @@ def test_the_stream_is_found_without_torchs_inner_function(monkeypatch):
         got = s.token_logprobs(x, top=4)
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got[1:], want[1:]))
+
+
+# ---- rows that share a wavefront, and the longest --------------------------------------------
+
+def _pick(v, keep):
+    return None if v is None else v[keep]
+
+
+@pytest.mark.parametrize('dtype', list(TYPES))
+@pytest.mark.parametrize('rows, cols', [(16385, 184), (16386, 256), (16387, 41), (8193, 1000), (8195, 520), (8193, 90)])
+def test_rows_that_share_wavefronts_with_some_left_over(rows, cols, dtype):
+    """Not a whole number of wavefronts; rows of every width next to each other, down to 0 and to fewer than the alternatives."""
+    s = _scores()
+    x = _rows(1, cols, dtype).expand(rows, cols).clone()
+    x += torch.randn(rows, cols, generator=torch.Generator().manual_seed(rows)).to(x.dtype).cuda()
+    x[5::97, ::3] = -math.inf
+    x[6::97] = -math.inf
+    x[7::97, cols // 2] = math.nan
+    widths = torch.randint(0, cols + 1, (rows,), generator=torch.Generator().manual_seed(cols), dtype=torch.int32)
+    widths[::5], widths[1::7], widths[2::9], widths[3::11] = 0, 1, 4, cols
+    keep = torch.cat([torch.arange(0, 60), torch.arange(rows - 40, rows)]).cuda()
+    for n, top, w in ((1, 0, None), (1, 5, None), (20, 8, None), (1, 5, widths.cuda()), (20, 8, widths.cuda()), (20, 0, widths.cuda()), (3, 14, widths.cuda())):
+        if top > 8 and rows > 16384:
+            continue
+        tokens = _tokens(rows, cols, n)
+        many = s.token_logprobs(x, tokens, top, w)
+        few = _check_logprobs(x[keep], tokens[keep], top, _pick(w, keep))
+        err = (cols / 64 + 96) * 2.0 ** -24 * (1 + math.log(cols + 1))
+        for a, b in zip(many, few):
+            if a is not None and a.dtype == torch.int32:
+                assert torch.equal(a[keep], b)
+            elif a is not None:
+                a, b = _np(a[keep]), _np(b)
+                assert np.array_equal(np.isfinite(a), np.isfinite(b)) and np.array_equal(a[~np.isfinite(a)], b[~np.isfinite(b)], equal_nan=True)
+                fine = np.isfinite(a)
+                # two results of other orders of adding, each off by at most err and 2 u of its value
+                assert (np.abs(a[fine] - b[fine]) <= 2 * err + 4 * 2.0 ** -24 * np.abs(b[fine])).all()
+
+
+def test_rows_of_the_most_columns():
+    cols = 1 << 24
+    x = torch.randn(2, cols, device='cuda', generator=torch.Generator('cuda').manual_seed(1)).bfloat16()
+    tokens = torch.tensor([[0, cols - 1], [cols, 77]], device='cuda')
+    x[0, cols - 1] = 9
+    widths = torch.tensor([cols, cols - 5], dtype=torch.int32, device='cuda')
+    r = _check_logprobs(x, tokens, 5, widths)
+    g = torch.ones(2, 2, device='cuda')
+    grad = _scores().token_logprobs_backward(x, r.stats, tokens, g, widths=widths)
+    p = torch.softmax(x[0].double(), 0)
+    want = -2 * p
+    want[0] += 1
+    want[-1] += 1
+    # bfloat16's half step, and the statistics' error times the value
+    assert ((grad[0].double() - want).abs() <= want.abs() * (2.0 ** -8 + (cols / 64 + 96) * 2.0 ** -24) + 2.0 ** -134).all()
+    assert not grad[1, cols - 5:].any()
+    with pytest.raises(ValueError):
+        _scores().token_logprobs(x[:1].expand(1, cols).as_strided((1, cols + 1), (cols + 1, 1)), top=1)
