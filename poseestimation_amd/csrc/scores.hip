@@ -132,7 +132,8 @@ __device__ __forceinline__ uint32_t sc_dpp(uint32_t v) {
     return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
 }
 
-// One step of a butterfly: p and q are v of the two neighbouring groups of STEP lanes, in the same order for both.
+// One step of a butterfly: p and q are v of the two neighbouring groups of STEP lanes.  Below 16 lanes p is a lane's own, so that
+// the two groups have them in opposite orders and what is made of them must not depend on it; from 16 on the order is the same.
 // Within a group of STEP lanes v is the same already, so that any lane of the other group will do: the row mirrors stand
 // in for the exchanges at 4 and 8, and the row swaps of v with itself give both sides at 16 and 32.  (An exchange through
 // LDS, as __shfl_xor, issues at a third of their rate.)
@@ -432,10 +433,12 @@ __device__ __forceinline__ float sc_kth_all(const float* f, int K, uint32_t lo, 
 
 // ---- 16, 32 or 64 lanes to the row: up to 2048 columns, all of them in registers ----------------
 //
-// Bound by instruction issue and latency, not by memory: some ten instructions a score, and a few hundred for the
-// reductions, the alternatives and the results, which the rows of a wavefront share.  So rows are packed as tightly as
-// their number allows; nothing is exchanged through LDS but the handful of candidates, and wavefronts do not wait for
-// each other.
+// Some ten instructions a score, and a few hundred for the reductions, the alternatives and the results, which the rows of a
+// wavefront share; so rows are packed as tightly as their number allows, nothing is exchanged through LDS but the handful of
+// candidates, and wavefronts do not wait for each other.  Bound by latency first, with few wavefronts to cover it: 16-bit rows
+// of 24 scores a lane take 107 registers, of 32 scores 125, which leaves four wavefronts to a SIMD, 4096 on the chip.  Issue is
+// 38 of 63 to 74 us at 65536 x 1000 bfloat16 (floor 26) and 4.5 of 14.5 at 9216 ragged rows of up to 656, whose 4608
+// wavefronts do not all start at once: 8192 rows take 10.8 us, 8448 13.8.
 
 #define SC_WAVE_CAND 128  // candidates of a wavefront's rows
 
@@ -502,7 +505,9 @@ __global__ __launch_bounds__(SC_WG) void k_token_logprobs_rows(LogprobArgs a) {
             count = sc_lanes(__popc(take), L, SumOp());
             if (!once || count <= room) break;
             // With many alternatives, or more than there are lanes in use, too many scores reach the lanes' bound (at 64 some
-            // 250 of 2048): it is taken on from there among all of them.
+            // 250 of 2048): it is taken on from there among all of them.  (Rows that share a wavefront are then done one
+            // alternative after the other, as below, which takes as long: 8000 x 100 with sixteen, a wavefront each, and 8192,
+            // two to one, 26 us both.)
             tau = sc_kth_all<N>(f, a.top, sc_order(tau), sc_order(st.m));
         }
         if (__any(count > room)) {
@@ -567,7 +572,9 @@ __global__ __launch_bounds__(SC_WG) void k_token_logprobs_rows(LogprobArgs a) {
 //
 // Chunks of WG * 32 columns, 32 to a thread in 16-byte loads.  With many rows: 64 or 256 threads, and workgroups enough on
 // a CU to keep the loads coming while others reduce; bound by the memory (4096 x 131072 bfloat16 with five alternatives:
-// 196 us, 5.5 TB/s).  With few long rows: 1024 threads that load a chunk while they add the one before; bound by
+// 196 us, 5.5 TB/s).  With 64 the LDS holds sixteen on a CU, 4096 on the chip: 4096 x 4096 takes 13 us, 4352 x 4096 15.6 and
+// 8192 x 4096 22 (floor 13).  With 256 a row of 16384 columns takes 1.6 us of its CU, and 5.6 to start and to end: 1400 of
+// them 15.5 us (floor 9), as long as 1536.  With few long rows: 1024 threads that load a chunk while they add the one before; bound by
 // instruction issue on the one CU (131072 columns 9 us) and by the latency of the steps behind the last load.  Still fewer
 // long rows are cut into slices, joined by k_token_logprobs_join.
 
@@ -727,7 +734,8 @@ struct Nothing {};
 template <typename X, int WG, bool TOP>
 __global__ __launch_bounds__(WG) void k_token_logprobs_block(LogprobArgs a) {
     constexpr int V = X::V, NV = SC_PER_THREAD / V, CHUNK = WG * SC_PER_THREAD, WAVES = WG / 64;
-    // few workgroups: nobody else to fill the time between a load and its use (float32: no registers for it)
+    // few workgroups: nobody else to fill the time between a load and its use (float32: with alternatives six registers too
+    // many; without them there is room, which is not taken)
     constexpr bool AHEAD = WG == 1024 && V == 8;
     __shared__ Stat wave_stat[WAVES];
     __shared__ typename std::conditional<TOP, TopShared<WG>, Nothing>::type sh;
@@ -876,8 +884,9 @@ struct LogprobGradArgs {
 };
 
 // dx_j = -p_j (sum g + gH (log p_j + H)) + the tokens' own g, with t = log2 p_j = (x_j - m) log2 e - log2 S:
-// one read and one write of the row, some eleven instructions a score, bound by the memory.  A lane holds a token
-// (n_tok <= 64), so that the row's scores are compared with none: the one lane that holds a token's column adds
+// one read and one write of the row, some eleven instructions a score, bound by the memory; short 16-bit rows by the number of
+// wavefronts, one to a row (bfloat16, 65536 x 40 24.5 us, x 128 25.8, x 1000 61, x 2000 120; floors 2, 6.7, 52, 104).  A lane holds
+// a token (n_tok <= 64), so that the row's scores are compared with none: the one lane that holds a token's column adds
 // its g before the value is rounded, the tokens in their order.
 struct GradRow {
     float base, log2_sum, c0, c1;  // dx = -p (c0 + c1 t)
@@ -1009,7 +1018,13 @@ __global__ __launch_bounds__(SC_WG) void k_token_logprobs_grad_block(LogprobGrad
 // group, a wavefront 64 / L rows.  A score and its place are one number, the place in mantissa bits that the score does not
 // use, so that one v_max orders both and no two are equal: bfloat16 and float16 logits leave 13 bits of 32, all else goes
 // into a float64 (whose v_max issues at the same rate).  A lane sorts its experts KP at a time by
-// a bitonic network, keeps the best KP, and the lanes merge theirs in log2 L exchanges.  Bound by instruction issue.
+// a bitonic network, keeps the best KP, and the lanes merge theirs in log2 L exchanges.
+//
+// 65536 x 128 bfloat16 to eight: 11.5 us, 3.4 of them the launch and the first rows' latency, the rest 0.11 to 0.13 us for 1024
+// rows, of which issue (630 instructions for eight rows) takes 0.08 and the bytes 0.06; the last 1024 of 8192 wavefronts wait
+// for a place (65 registers leave seven to a SIMD): 0.6 us.  By p + bias and in groups issue is 36 of 57 us at 65536 x 256 (1697
+// instructions for four rows), and three wavefronts a SIMD (161 registers) cover the latency badly.  Groups with the same sum
+// go to float64, 5 us of a wavefront for a row: 65536 x 256 equal logits 277 us, a tenth of the rows equal 91.
 
 struct RouteArgs {
     const void* x;
@@ -1509,7 +1524,8 @@ struct RouteGradArgs {
 //                              chosen; 0 elsewhere, and the other logits are not read;
 //   softmax as it is:          dx_j = p_j ([j chosen] g_j - sum over the chosen of g_i p_i), which reaches every expert.
 // A row's lanes put the chosen experts' values into the row's zeroes in LDS (an expert named twice adds up) and write it out
-// in 16-byte pieces.  Bound by the memory and the latency of index -> logit.
+// in 16-byte pieces.  Bound by the memory and the latency of index -> logit; the softmax as it is (32768 x 160 9 to 10 us, floor
+// 4.5) also by its 74 registers, six wavefronts a SIMD: 24576 rows, which all find a place, take 6.8 us, 28672 8.4.
 template <typename X, int NV, bool DENSE>
 __global__ __launch_bounds__(SC_WG) void k_route_grad(RouteGradArgs a) {
     constexpr int V = X::V;
@@ -1724,7 +1740,7 @@ static void sc_launch_logprobs(const LogprobArgs& a, int wg_size, hipStream_t st
             hipLaunchKernelGGL((k_token_logprobs_rows<X, 3>), grid, wg, 0, stream, a);
         else if (vecs <= 4)
             hipLaunchKernelGGL((k_token_logprobs_rows<X, 4>), grid, wg, 0, stream, a);
-        else if (vecs <= 6)
+        else if (vecs <= 6)  // float32 from here on: 16-bit rows have four at most
             hipLaunchKernelGGL((k_token_logprobs_rows<X, 24 / X::V>), grid, wg, 0, stream, a);
         else
             hipLaunchKernelGGL((k_token_logprobs_rows<X, 32 / X::V>), grid, wg, 0, stream, a);
